@@ -1,0 +1,275 @@
+"""GPU tests of the network-side operators (include/umr_nn.h): the kernels at sizes that take every route through them, and
+umr_amd.functional's linear_act / heads_linear_act / balance_loss as a user calls them."""
+import pytest
+import torch
+
+import host_nn as H
+import nn_checks as C
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _lib():
+    from umr_amd import _lib
+    return _lib.lib()
+
+
+# few rows (one, two, four row blocks; split and not; odd rows in memory), tiles of 64 and 128 (edges in each direction, split), heads
+LINEAR = [(1, 1, 200, 200, 0), (1, 1, 1, 1, 0), (16, 1, 200, 4096, 0), (5, 3, 1011, 350, 3), (31, 1, 515, 2047, 1), (64, 2, 130, 700, 8),
+          (65, 1, 129, 65, 1), (777, 1, 301, 515, 13), (1000, 1, 1011, 350, 0), (2500, 1, 2049, 130, 0), (130, 9, 200, 200, 0),
+          (70, 1, 5, 20000, 0), (20000, 1, 7, 3, 0), (300, 1, 7, 0, 0)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M,G,N,K,pad", LINEAR)
+def test_linear_against_64_bits(M, G, N, K, pad, dtype):
+    C.check_linear(_lib(), M, G, N, K, dtype, "silu", device=DEV, pad=pad)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("act", list(H.ACT))
+def test_linear_activations(act, dtype):
+    C.check_linear(_lib(), 33, 2, 70, 64, dtype, act, device=DEV)
+    C.check_linear(_lib(), 200, 1, 70, 64, dtype, act, device=DEV, bias=False, residual=False)
+
+
+BALANCE = [(1, 1, 1, "none"), (16, 8, 1, "none"), (5001, 61, 2, "both"), (70000, 128, 8, "rows"), (3000, 1000, 3, "choices"), (40000, 3, 2, "both"),
+           (640, 16, 4, "nothing"), (0, 7, 1, "none"), (9000, 257, 1, "both"), (1025, 513, 2, "rows")]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("T,E,k,mask", BALANCE)
+def test_balance_against_64_bits(T, E, k, mask, dtype):
+    C.check_balance(_lib(), T, E, k, dtype, mask, device=DEV)
+
+
+def _layer64(x, w, b, r, act, slope, gy):
+    """z, the sum of the magnitudes that enter it, y and dz in 64 bits"""
+    x, w, b, r, gy = (t.detach().double() for t in (x, w, b, r, gy))
+    z = torch.einsum("mgk,gnk->mgn", x, w) + b
+    zmag = torch.einsum("mgk,gnk->mgn", x.abs(), w.abs()) + b.abs()
+    y = C.act64(z, act, slope) + r
+    dz = gy * C.act_slope64(z, act, slope)
+    return z, zmag, y, dz
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("act", ["none", "tanh", "gelu", "silu"])
+@pytest.mark.parametrize("M,G,N,K", [(1, 4, 200, 200), (16, 8, 200, 200), (100, 3, 65, 130), (3, 1, 9, 4)])
+def test_layers_and_their_gradients(M, G, N, K, act, dtype):
+    """heads_linear_act on strided inputs, every gradient through autograd, full and one-row residual; linear_act on the heads that share
+    their input"""
+    from umr_amd import functional as UF
+    x, w, b, r, gy = C.inputs(M, G, N, K, dtype, DEV, pad=3)
+    z, zmag, y64, dz64 = _layer64(x, w, b, r, act, 0.0, gy)
+    U, e = C.U, C.half_step(dtype)
+    ztol = (K + 2) * U * zmag
+    ytol = 1.13 * ztol + 16 * U * (z.abs() + 1) + U * (y64.abs() + 2 * r.double().abs())
+    # dz: |act''| <= 0.8 on the error of z, the evaluation of act', one rounding to the type (none without an activation)
+    dtol = torch.zeros_like(z) if act == "none" else gy.double().abs() * (0.8 * ztol + 32 * U * (z.abs() + 1)) + e * dz64.abs()
+    x64, w64 = x.double(), w.double()
+    dmag = dz64.abs() + dtol
+    want = dict(x=(torch.einsum("mgn,gnk->mgk", dz64, w64), torch.einsum("mgn,gnk->mgk", dtol + (N + 2) * U * dmag, w64.abs())),
+                w=(torch.einsum("mgn,mgk->gnk", dz64, x64), torch.einsum("mgn,mgk->gnk", dtol + (M + 2) * U * dmag, x64.abs())),
+                b=(dz64.sum(0), (dtol + (M + 2) * U * dmag).sum(0)))
+    for one_row in (False, True):
+        leaves = dict(x=x, w=w, b=b, r=(r[0] if one_row else r))
+        leaves = {k: v.detach().requires_grad_(True) for k, v in leaves.items()}
+        y = UF.heads_linear_act(leaves["x"], leaves["w"], leaves["b"], residual=leaves["r"], activation=act)
+        res = r[:1].expand_as(r).double() if one_row else r.double()
+        C.close(y.detach(), y64 - r.double() + res, ytol + U * res.abs(), "y")
+        grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), gy)))
+        for name in want:
+            C.close(grads[name], *want[name], name)
+        if one_row:
+            C.close(grads["r"], gy.double().sum(0), (M + 2) * U * gy.double().abs().sum(0), "r")
+        else:
+            assert torch.equal(grads["r"], gy)
+    # heads that share their input are one layer
+    shared = x[:, 0]
+    y = UF.linear_act(shared, w.flatten(0, 1), b.flatten(), activation=act).unflatten(-1, (G, N))
+    per = UF.heads_linear_act(shared.unsqueeze(1).expand(M, G, K), w, b, activation=act)
+    tol = 2 * (1.13 * (K + 2) * U * (torch.einsum("mk,gnk->mgn", shared.double().abs(), w64.abs()) + b.double().abs()) + 16 * U * (z.abs().amax() + 1))
+    C.close(y, per.double(), tol + e * per.double().abs(), "shared input")
+
+
+def test_leading_dimensions_strides_and_one_row():
+    from umr_amd import functional as UF
+    g = torch.Generator(device=DEV).manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, device=DEV, generator=g)
+    x, w, b = rnd(4, 5, 6, 24), rnd(10, 24), rnd(10)
+    flat = UF.linear_act(x.reshape(-1, 24), w, b, activation="relu")
+    assert torch.equal(UF.linear_act(x, w, b, activation="relu").reshape(-1, 10), flat)
+    for view in (x.transpose(0, 1), x[:, ::2], x.permute(2, 0, 1, 3), x[..., None, :].expand(4, 5, 6, 3, 24)):
+        assert torch.equal(UF.linear_act(view, w, b, activation="relu"), UF.linear_act(view.contiguous(), w, b, activation="relu"))
+    wt = rnd(24, 10).t()                                                    # weight whose columns lie together
+    assert torch.equal(UF.linear_act(x, wt), UF.linear_act(x, wt.contiguous()))
+    xt = rnd(24, 30).t()
+    assert torch.equal(UF.linear_act(xt, w), UF.linear_act(xt.contiguous(), w))
+    one = UF.linear_act(x[0, 0, 0], w, b, residual=b)                       # a vector in, a vector out
+    assert one.shape == (10,) and torch.equal(one, UF.linear_act(x[0, 0, :1], w, b, residual=b)[0])
+    assert UF.linear_act(x[:0], w, b).shape == (0, 5, 6, 10)
+    # the gradient of a broadcast: one number for all outputs; no rows: zeros
+    wl, xl = w.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    gs = torch.autograd.grad(UF.linear_act(xl, wl, activation="tanh").sum(), [xl, wl])
+    ge = torch.autograd.grad(UF.linear_act(xl, wl, activation="tanh"), [xl, wl], torch.ones(4, 5, 6, 10, device=DEV))
+    assert all(torch.equal(a, c) for a, c in zip(gs, ge))
+    y = UF.linear_act(xl[:0], wl, activation="gelu")
+    gx, gw = torch.autograd.grad(y.sum(), [xl, wl])
+    assert bool((gx == 0).all()) and bool((gw == 0).all())
+    # an input that needs no gradient gets none, and the others are the same bits
+    only = torch.autograd.grad(UF.linear_act(x, wl, activation="tanh"), [wl], torch.ones(4, 5, 6, 10, device=DEV))[0]
+    assert torch.equal(only, ge[1])
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(UF.linear_act(xl, wl, activation="tanh").sum(), wl, create_graph=True)
+
+
+def test_kinked_activations_keep_only_a_sign():
+    """relu and leaky relu: without a residual the output serves the backward call, with one a copy of z does; 0 counts as negative"""
+    from umr_amd import functional as UF
+    x = torch.tensor([[-2.0], [0.0], [3.0]], device=DEV, requires_grad=True)
+    w, r = torch.ones(1, 1, device=DEV), torch.full((3, 1), 5.0, device=DEV)
+    for act, want in (("relu", [0.0, 0.0, 1.0]), ("leaky_relu", [0.25, 0.25, 1.0])):
+        for res in (None, r):
+            y = UF.linear_act(x, w, residual=res, activation=act, slope=0.25)
+            assert torch.autograd.grad(y.sum(), x)[0].flatten().tolist() == want
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y = UF.linear_act(x, w, activation="relu")
+        y.add_(1)
+        y.sum().backward()
+
+
+def test_offsets_beyond_32_bits():
+    """outputs, weights and rows more than 2^31 elements in: the far ends against the same rows computed alone"""
+    from umr_amd import functional as UF
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.randn(70001, 24, device=DEV, generator=g).bfloat16()
+    w = torch.randn(33000, 24, device=DEV, generator=g).bfloat16()
+    y = UF.linear_act(x, w, activation="leaky_relu", slope=0.1)              # 2.3e9 outputs
+    tail = UF.linear_act(x[-3:].clone(), w[-40:].clone(), activation="leaky_relu", slope=0.1)
+    C.close(y[-3:, -40:].contiguous(), tail.double(), 52 * C.U * (x[-3:].double().abs() @ w[-40:].double().abs().t()) + 2.0 ** -8 * tail.double().abs(), "far outputs")
+    gy = torch.zeros_like(y)
+    gy[-1, -5:] = 1
+    xl = x.clone().requires_grad_(True)
+    gx, = torch.autograd.grad(UF.linear_act(xl, w), xl, gy)                  # reads the far end of a 2.3e9 gradient
+    want = w[-5:].double().sum(0)
+    C.close(gx[-1], want, 40000 * C.U * w[-5:].double().abs().sum(0), "dx of the last row")
+    assert bool((gx[:-1] == 0).all())
+    del y, gy, gx
+    big = torch.zeros(3, 1 << 30, device=DEV, dtype=torch.bfloat16)          # rows 2^30 apart: the third is 2^31 elements in
+    rows = big[:, :40]
+    rows.copy_(torch.randn(3, 40, device=DEV, generator=g))
+    w = torch.randn(7, 40, device=DEV, generator=g).bfloat16()
+    assert torch.equal(UF.linear_act(rows, w), UF.linear_act(rows.contiguous(), w))
+    assert torch.equal(UF.linear_act(w, rows), UF.linear_act(w, rows.contiguous()))
+    del big, rows
+    T = (1 << 31) // 64 + 5
+    z = torch.zeros(T, 64, device=DEV, dtype=torch.bfloat16)
+    z[-1, 3] = 40
+    inds = torch.zeros(T, 1, device=DEV, dtype=torch.int64)
+    inds[-1] = 3
+    loss, counts = UF.balance_loss(z.requires_grad_(True), inds)
+    assert counts[0] == T - 1 and counts[3] == 1
+    assert abs(float(loss.detach()) - 1.0) < 1e-4
+    dz, = torch.autograd.grad(loss, z, torch.tensor(float(T), device=DEV))
+    assert float(dz[-1].abs().sum()) < 1e-6 and bool((dz[-2] == dz[0]).all()) and float(dz[0, 0]) > 0
+
+
+def _capture(fn):
+    """fn's first runs on a side stream, then captured"""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            fn()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fn()
+    return graph, out
+
+
+def test_streams_and_graphs():
+    """forward and backward of the operators on another stream, and captured: two graphs replayed in turn with eager work between them,
+    every replay against the eager result on that replay's inputs"""
+    from umr_amd import functional as UF
+
+    def make(M, N, K, seed):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        x = torch.randn(M, K, device=DEV, generator=g).requires_grad_(True)
+        w = (torch.randn(N, K, device=DEV, generator=g) / 30).requires_grad_(True)
+        b = torch.randn(N, device=DEV, generator=g).requires_grad_(True)
+        r = torch.randn(N, device=DEV, generator=g).requires_grad_(True)
+        inds = torch.randint(0, N, (M, 2), device=DEV, generator=g)
+
+        def step():
+            y = UF.linear_act(x, w, b, residual=r, activation="gelu")
+            loss, counts = UF.balance_loss(y, inds)
+            return [loss.detach(), counts, y.detach()] + list(torch.autograd.grad(loss + (y * y).mean(), [x, w, b, r]))
+        return x, step
+    cases = [make(16, 200, 4096, 1), make(700, 60, 900, 2)]                # split contractions and many-row sums: every workspace
+    graphs = [_capture(step) for _, step in cases]
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    for turn in range(4):
+        for (x, step), (graph, out) in zip(cases, graphs):
+            with torch.no_grad():
+                x.copy_(torch.randn(x.shape, device=DEV, generator=gen))
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                eager = step()
+            torch.cuda.current_stream().wait_stream(side)
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, c in zip(eager, out):
+                assert torch.equal(a, c), turn
+    again = [step() for _, step in cases]
+    for (x, step), first in zip(cases, again):
+        assert all(torch.equal(a, c) for a, c in zip(first, step()))
+
+
+def test_registered_operators_pass_opcheck():
+    import umr_amd.ops_nn  # noqa: F401
+    from torch.library import opcheck
+    x, w, b, r, gy = C.inputs(5, 2, 6, 7, torch.float32, DEV)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (x, w, b, r)]
+    utils = ("test_schema", "test_autograd_registration", "test_faketensor")
+    opcheck(torch.ops.umr.linear_act, (*leaves, 4, 0.0), test_utils=utils)
+    opcheck(torch.ops.umr.linear_act_backward, (gy.clone(), x, w, gy.clone(), 4, 0.0, True, True, True, True), test_utils=utils)
+    z, inds, m = C.balance_inputs(9, 5, 2, torch.float32, DEV, "both")
+    opcheck(torch.ops.umr.balance_loss, (z.requires_grad_(True), inds, m), test_utils=utils)
+
+
+def test_a_routers_operators_together():
+    """As they are used: a layer that every head shares, a layer of each head's own, one score a head, the softmax's choice, the balance
+    loss over the heads; loss, counts and every gradient against the same in 64 bits, fp32 and 16 bits"""
+    from umr_amd import functional as UF
+    B, G, D = 64, 8, 200
+    for dtype in (torch.float32, torch.bfloat16):
+        gen = torch.Generator(device=DEV).manual_seed(4)
+        rnd = lambda *s: torch.randn(*s, device=DEV, generator=gen)
+        leaves = [t.to(dtype).requires_grad_(True) for t in (rnd(B, D), rnd(G * D, D) / D ** 0.5, 0.1 * rnd(G * D), rnd(G, 1, D) / D ** 0.5, 0.1 * rnd(G, 1))]
+        x, w1, b1, w2, b2 = leaves
+        hidden = UF.linear_act(x, w1, b1, activation="silu").unflatten(-1, (G, D))
+        scores = UF.heads_linear_act(hidden, w2, b2)[..., 0]
+        inds = torch.randint(0, G, (B, 1), device=DEV, generator=gen)
+        loss, counts = UF.balance_loss(scores, inds)
+        grads = torch.autograd.grad(loss, leaves, torch.tensor(float(B), device=DEV))
+        d = [t.detach().double().requires_grad_(True) for t in leaves]
+        h = torch.nn.functional.silu(d[0] @ d[1].t() + d[2]).unflatten(-1, (G, D))
+        s = torch.einsum("bgd,gd->bg", h, d[3][:, 0]) + d[4][:, 0]
+        c64 = torch.bincount(inds[:, 0], minlength=G)
+        l64 = G * torch.dot(c64.double() / B, torch.softmax(s, 1).mean(0))
+        g64 = torch.autograd.grad(l64, d, torch.tensor(float(B), device=DEV).double())
+        assert torch.equal(counts, c64)
+        # hidden, scores, d scores, d hidden and the gradients are each rounded to the type once; each rounding enters a gradient with
+        # a factor of at most 2 in the 2-norm (softmax, silu and the products of unit variance here do not enlarge it), fp32 sums of
+        # up to 1600 terms add 1600 u
+        tol = 10 * C.half_step(dtype) + 1600 * C.U
+        assert abs(float(loss.detach()) - float(l64)) <= tol * float(l64)
+        for a, c in zip(grads, g64):
+            assert float((a.double() - c).norm()) <= tol * float(c.norm())

@@ -77,6 +77,21 @@ SIGNATURES = {
     "umr_masked_l1_backward": ([_P, _P, _P, _P, _P, _P, _P, _I, _I, _L, _P], _I),
 }
 
+# the same for include/umr_nn.h
+SIGNATURES_NN = {
+    "umr_linear_forward_workspace_bytes": ([_L, _L, _L, _I, _I], _Z),
+    "umr_linear_forward": ([_P, _L, _L, _P, _L, _L, _P, _P, _L, _L, _P, _P, _L, _L, _L, _I, _I, _I, _F, _P, _Z, _P], _I),
+    "umr_linear_grad_act_workspace_bytes": ([_L, _L, _I], _Z),
+    "umr_linear_grad_act": ([_P, _L, _L, _P, _P, _P, _P, _L, _L, _I, _I, _I, _F, _P, _Z, _P], _I),
+    "umr_linear_grad_input_workspace_bytes": ([_L, _L, _L, _I, _I], _Z),
+    "umr_linear_grad_input": ([_P, _L, _L, _P, _L, _L, _P, _L, _L, _L, _I, _I, _P, _Z, _P], _I),
+    "umr_linear_grad_weight_workspace_bytes": ([_L, _L, _L, _I, _I], _Z),
+    "umr_linear_grad_weight": ([_P, _L, _L, _P, _L, _L, _P, _L, _L, _L, _I, _I, _P, _Z, _P], _I),
+    "umr_balance_workspace_bytes": ([_L, _I], _Z),
+    "umr_balance_forward": ([_P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _P, _Z, _P], _I),
+    "umr_balance_backward": ([_P, _P, _P, _P, _P, _L, _I, _I, _P], _I),
+}
+
 _lib = None
 
 
@@ -91,7 +106,7 @@ def lib():
         h = ctypes.CDLL(LIB_PATH)
         h.umr_version.restype = ctypes.c_char_p
         h.umr_build_id.restype = ctypes.c_char_p
-        for name, (argtypes, restype) in SIGNATURES.items():
+        for name, (argtypes, restype) in list(SIGNATURES.items()) + list(SIGNATURES_NN.items()):
             fn = getattr(h, name)
             fn.argtypes = argtypes
             fn.restype = restype

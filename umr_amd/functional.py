@@ -741,6 +741,67 @@ def masked_l1(img_pred, img_gt, mask_gt, mask_pred):
     return _ops(img_pred, img_gt, mask_gt, mask_pred).masked_l1(img_pred, img_gt, mask_gt, mask_pred)
 
 
+# ------------------------------------------------------------------------------------------------------------------------
+# The network side (csrc/linear.hip, csrc/balance.hip; operators in csrc/torch_nn.cpp).
+_nn = None
+
+
+def _nn_ops(*tensors):
+    """(torch.ops.umr, ops_nn), after refusing host tensors as _ops does."""
+    global _nn
+    if _nn is None:
+        from . import ops_nn
+        _nn = (torch.ops.umr.linear_act.default, torch.ops.umr.balance_loss.default, ops_nn.ACTIVATIONS)
+    for t in tensors:
+        if torch.is_tensor(t) and not (t.is_cuda or t.is_meta):
+            raise RuntimeError("umr_amd: expected a GPU tensor, got %s (no CPU path exists)" % t.device)
+    return _nn
+
+
+def _activation(table, name):
+    if name not in table:
+        raise ValueError("umr_amd: activation must be one of %s, got %r" % (", ".join(table), name))
+    return table[name]
+
+
+def linear_act(x, weight, bias=None, residual=None, activation="none", slope=0.01):
+    """act(x @ weight.T + bias) + residual in one kernel (two where the product is split along K): x [.., K], weight [N, K], bias
+    [N], residual [.., N] or one row [N] for all -> [.., N].  activation: none, relu, leaky_relu (slope >= 0), tanh, gelu (the
+    exact form), silu.
+
+    float32, bfloat16 or float16, one type for all; sums are fp32 and a result is rounded once.  Any strides: rows that are
+    contiguous are read in place, whatever lies between them.  Gradients to x, weight, bias and residual (in 16 bits the gradient of the
+    pre-activation is rounded to 16 bits, as the operands of the matrix unit are); at a kink the derivative is the negative
+    side's.  Not differentiable twice.  The same inputs give the same bits in every call."""
+    op, _, table = _nn_ops(x, weight, bias, residual)
+    if weight.dim() != 2:
+        raise RuntimeError("umr_amd: linear_act: weight must be [N, K], got %s" % list(weight.shape))
+    return op(x, weight, bias, residual, _activation(table, activation), slope)
+
+
+def heads_linear_act(x, weight, bias=None, residual=None, activation="none", slope=0.01):
+    """linear_act for G heads at once, each with a layer of its own: x [.., G, K], weight [G, N, K], bias [G, N], residual
+    [.., G, N] or [G, N] -> [.., G, N].  (Heads that share their input are one layer: linear_act with weight.flatten(0, 1), its
+    output unflattened.)"""
+    op, _, table = _nn_ops(x, weight, bias, residual)
+    if weight.dim() != 3:
+        raise RuntimeError("umr_amd: heads_linear_act: weight must be [G, N, K], got %s" % list(weight.shape))
+    return op(x, weight, bias, residual, _activation(table, activation), slope)
+
+
+def balance_loss(scores, inds, mask=None):
+    """-> (loss, counts): how unevenly E choices are used.  scores [T, E] (before the softmax; float32, bfloat16 or float16),
+    inds [T, k] int64: the choices that were taken, mask [T] bool: rows that count (None: all).
+
+        loss = E sum_e f_e P_e,   f_e = counts[e] / (n k),   P_e = mean of softmax(scores)[:, e],   over the n rows that count
+
+    loss is a float32 scalar, 1 when all choices are used alike, differentiable in scores (through P; counts are constants);
+    counts [E] int64.  A score of -inf is never chosen; a row of nothing else counts as masked out; masked rows may hold
+    anything.  An index outside 0 .. E-1 counts for no choice, one that appears twice counts twice.  E <= 1024."""
+    _, op, _ = _nn_ops(scores, inds, mask)
+    return op(scores, inds, mask)
+
+
 class _Apply:
     def __init__(self, fn):
         self.apply = fn
