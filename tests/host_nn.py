@@ -12,7 +12,7 @@ ROOT = os.path.dirname(HERE)
 CLANG = "/opt/rocm/lib/llvm/bin/clang++"
 SRC_DIR = os.path.join(HERE, "host_kernel")
 SO = os.path.join(SRC_DIR, "libumr_nn_host.so")
-TUS = ["linear", "balance"]
+TUS = ["linear", "linear_f32", "linear_bf16", "linear_f16", "balance"]
 DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACT = {"none": 0, "relu": 1, "leaky_relu": 2, "tanh": 3, "gelu": 4, "silu": 5}
 

@@ -16,7 +16,7 @@ TORCH_LIB = os.path.join(LIBDIR, "libumr_torch.so")
 SOURCES = ["raster.hip", "geometry.hip", "losses.hip", "perceptual.hip", "edt.hip", "atlas.hip", "regs.hip", "eval.hip"]
 # The network-side operators, compiled without packed fp32 instructions: some forms of v_pk_{add,mul,fma}_f32 that the compiler
 # makes from ordinary float code have given wrong results on this target now and then.
-NN_SOURCES = ["linear.hip", "balance.hip"]
+NN_SOURCES = ["linear.hip", "linear_f32.hip", "linear_bf16.hip", "linear_f16.hip", "balance.hip"]
 NN_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-shared",

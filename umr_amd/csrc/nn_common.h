@@ -70,6 +70,48 @@ template <class T> f32x16 mma32(T, u32x4 a, u32x4 b, f32x16 c);
 template <class T> f32x4 mma16(T, u32x4 a, u32x4 b, f32x4 c);
 #endif
 
+// Steps of a butterfly over the 2, 4 .. 64 lanes of a row: the partner's value, where a step may take any lane of the partner's group
+// because the groups of O lanes already agree (O = 4, 8: the mirrored lane).  Up to 16 lanes these are DPP moves, without LDS.
+template <int O> __device__ __forceinline__ float across(float v) {
+#ifndef UMR_HOST_SHIM
+    constexpr int ctrl = O == 1 ? 0xB1 /* quad_perm 1,0,3,2 */ : O == 2 ? 0x4E /* 2,3,0,1 */ : O == 4 ? 0x141 /* half mirror */ : 0x140 /* mirror */;
+    if constexpr (O <= 8) return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xf, 0xf, true));
+#endif
+    return __shfl_xor(v, O, UMR_WAVE);
+}
+template <int N> __device__ __forceinline__ float group_sum(float v) {          // over groups of N lanes; every lane gets it
+    if constexpr (N >= 2) v += across<1>(v);
+    if constexpr (N >= 4) v += across<2>(v);
+    if constexpr (N >= 8) v += across<4>(v);
+    if constexpr (N >= 16) v += across<8>(v);
+    if constexpr (N >= 32) v += across<16>(v);
+    if constexpr (N >= 64) v += across<32>(v);
+    return v;
+}
+template <int N> __device__ __forceinline__ float group_max(float v) {          // NaN is left out
+    if constexpr (N >= 2) v = fmaxf(v, across<1>(v));
+    if constexpr (N >= 4) v = fmaxf(v, across<2>(v));
+    if constexpr (N >= 8) v = fmaxf(v, across<4>(v));
+    if constexpr (N >= 16) v = fmaxf(v, across<8>(v));
+    if constexpr (N >= 32) v = fmaxf(v, across<16>(v));
+    if constexpr (N >= 64) v = fmaxf(v, across<32>(v));
+    return v;
+}
+__device__ __forceinline__ float exp2_of(float x) {      // one v_exp_f32: results below 2^-126 are 0
+#ifndef UMR_HOST_SHIM
+    return __builtin_amdgcn_exp2f(x);
+#else
+    return exp2f(x);
+#endif
+}
+
+// Nothing is scheduled across: loads that were written ahead of the matrix instructions stay ahead of them.
+#ifndef UMR_HOST_SHIM
+#define UMR_SCHED_FENCE() __builtin_amdgcn_sched_barrier(0)
+#else
+#define UMR_SCHED_FENCE() ((void)0)
+#endif
+
 // Loads at the element's own alignment: this target's global loads take any, so rows of odd length need no other kernel.
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef u32x2 u32x2_any __attribute__((aligned(2)));
@@ -128,4 +170,12 @@ template <class T> __device__ __forceinline__ void store4(T *p, long n, const fl
         for (int i = 0; i < 4; ++i)
             if (i < n) p[i] = from_f32<T>(v[i]);
     }
+}
+
+// 4 bytes of a result; STREAM: past the caches
+template <bool STREAM, class T> __device__ __forceinline__ void store_word(T *p, unsigned v) {
+#ifndef UMR_HOST_SHIM
+    if constexpr (STREAM) { __builtin_nontemporal_store(v, (u32_any *)p); return; }
+#endif
+    *(u32_any *)p = v;
 }
