@@ -13,50 +13,49 @@
 
 namespace {
 
-constexpr int WG = 256;
+constexpr int WG = 256, ROWS_WG = 1024;                  // threads of a workgroup, backward and forward
 
 template <class T, int LPR, int J> struct Row {          // one row's pieces in LPR lanes: lane s holds elements (j LPR + s) V .. + V
     static constexpr int V = 16 / (int)sizeof(T);
-    float p[J][V];
+    float x[J][V], r;                                    // softmax = x r
 
-    // the row's scores, then its softmax; false: nothing to choose from (every score -inf)
+    // false: nothing to choose from (every score -inf)
     __device__ __forceinline__ bool softmax(const T *z, int E, int s) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int e0 = (j * LPR + s) * V;
             const u32x4 v = load16B_n(z + e0, E - e0);
 #pragma unroll
-            for (int i = 0; i < V; ++i) p[j][i] = e0 + i < E ? elem_of<T>(v, i) : -INFINITY;
+            for (int i = 0; i < V; ++i) x[j][i] = e0 + i < E ? elem_of<T>(v, i) : -INFINITY;
         }
-        float m = -INFINITY;                             // (fmaxf leaves a NaN out; it comes back through the exponentials)
-        bool some = false;
+        float m = -INFINITY;                             // (a NaN is left out; it comes back through the exponentials)
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int i = 0; i < V; ++i) { m = fmaxf(m, p[j][i]); some |= p[j][i] != -INFINITY; }
-        int any = some;
+            for (int i = 0; i < V; ++i) m = fmaxf(m, x[j][i]);
+        m = group_max<LPR>(m);
+        float none = 0.f;
+        if (__any(m == -INFINITY)) {                     // a row without a maximum: all -inf, or NaN among them
+            float nans = 0.f;
 #pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) { m = fmaxf(m, __shfl_xor(m, o, UMR_WAVE)); any |= __shfl_xor(any, o, UMR_WAVE); }
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i) nans += x[j][i] != x[j][i] ? 1.f : 0.f;
+            nans = group_sum<LPR>(nans);                 // (every lane takes part)
+            none = m == -INFINITY && nans == 0.f ? 1.f : 0.f;
+        }
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                // 2^((z - m) log2 e): off by |z - m| 2^-24 of its value and half a unit of the exponential, i.e. far below 2^-24 of
-                // the row's sum wherever |z - m| is large
-                p[j][i] = exp2f((p[j][i] - m) * 1.44269504088896341f);
-                const int e = (j * LPR + s) * V + i;
-                if (e >= E) p[j][i] = 0.f;
-                sum += p[j][i];
+                // 2^((x - m) log2 e): off by |x - m| 2^-24 of its value and a unit of the exponential, i.e. far below 2^-24 of the
+                // row's sum wherever |x - m| is large.  Behind the row's end: exp(-inf) = 0.
+                x[j][i] = exp2_of((x[j][i] - m) * 1.44269504088896341f);
+                sum += x[j][i];
             }
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, UMR_WAVE);
-        const float r = 1.f / sum;
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-#pragma unroll
-            for (int i = 0; i < V; ++i) p[j][i] *= r;
-        return any != 0;
+        r = 1.f / group_sum<LPR>(sum);
+        return none == 0.f;
     }
 };
 
@@ -87,13 +86,13 @@ __device__ __forceinline__ void finish(const double *usage, const int *count, lo
 }
 
 template <class T, int LPR, int J>
-__global__ __launch_bounds__(WG) void k_balance_rows(const T *z, const long long *inds, const unsigned char *mask, float *part_p, int *part_c,
+__global__ __launch_bounds__(ROWS_WG) void k_balance_rows(const T *z, const long long *inds, const unsigned char *mask, float *part_p, int *part_c,
                                                      float *loss, long long *counts, float *coef, long T_rows, int E, int k, long rows) {
     constexpr int V = 16 / (int)sizeof(T), RPW = 64 / LPR, W = LPR * V * J;      // rows per wave, columns a row's lanes hold (>= E)
-    __shared__ float usage[WG / 64][W];
+    __shared__ float usage[ROWS_WG / 64][W];
     __shared__ int hist[W + 1];                                                  // [E]: the number of valid rows
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, s = lane % LPR, sub = lane / LPR;
-    for (int e = t; e < W + 1; e += WG) hist[e] = 0;
+    for (int e = t; e < W + 1; e += ROWS_WG) hist[e] = 0;
     __syncthreads();
     const long r0 = blockIdx.x * rows, r1 = r0 + rows < T_rows ? r0 + rows : T_rows;
     float acc[J][V];
@@ -101,7 +100,7 @@ __global__ __launch_bounds__(WG) void k_balance_rows(const T *z, const long long
     for (int j = 0; j < J; ++j)
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[j][i] = 0.f;
-    for (long b = r0 + wave * RPW; b < r1; b += RPW * (WG / 64)) {               // (uniform per wave: the butterflies need every lane)
+    for (long b = r0 + wave * RPW; b < r1; b += RPW * (ROWS_WG / 64)) {               // (uniform per wave: the butterflies need every lane)
         const long row = b + sub;
         const bool here = row < r1;
         const long safe = here ? row : r1 - 1;
@@ -111,7 +110,7 @@ __global__ __launch_bounds__(WG) void k_balance_rows(const T *z, const long long
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[j][i] += r.p[j][i];
+            for (int i = 0; i < V; ++i) acc[j][i] = fmaf(r.x[j][i], r.r, acc[j][i]);
         if (s == 0) atomicAdd(&hist[W], 1);
         for (int i = s; i < k; i += LPR) {
             const long long e = inds[row * k + i];
@@ -128,26 +127,42 @@ __global__ __launch_bounds__(WG) void k_balance_rows(const T *z, const long long
         }
     __syncthreads();
     if (part_p) {
-        for (int e = t; e < E; e += WG) {
+        for (int e = t; e < E; e += ROWS_WG) {
             float v = usage[0][e];
 #pragma unroll
-            for (int w = 1; w < WG / 64; ++w) v += usage[w][e];
+            for (int w = 1; w < ROWS_WG / 64; ++w) v += usage[w][e];
             part_p[(long)blockIdx.x * E + e] = v;
             part_c[(long)blockIdx.x * (E + 1) + e] = hist[e];
         }
         if (t == 0) part_c[(long)blockIdx.x * (E + 1) + E] = hist[W];
         return;
     }
-    __shared__ double sums[W], red[WG];
-    __shared__ long all[WG];                                          // the only workgroup: finish here
-    for (int e = t; e < E; e += WG) {
+    __shared__ double sums[W], red[ROWS_WG];
+    __shared__ long all[ROWS_WG];                                          // the only workgroup: finish here
+    for (int e = t; e < E; e += ROWS_WG) {
         double v = 0.0;
 #pragma unroll
-        for (int w = 0; w < WG / 64; ++w) v += usage[w][e];
+        for (int w = 0; w < ROWS_WG / 64; ++w) v += usage[w][e];
         sums[e] = v;
     }
     __syncthreads();
     finish(sums, hist, hist[W], loss, counts, coef, E, k, red, all);
+}
+
+// Many parts first become one of 32, in part order: read by one workgroup alone, 512 parts of 128 choices took 28 us.
+constexpr int FOLD = 32;
+__global__ __launch_bounds__(256) void k_balance_fold(const float *part_p, const int *part_c, int blocks, float *to_p, int *to_c, int E) {
+    const int b0 = blockIdx.x * FOLD, b1 = b0 + FOLD < blocks ? b0 + FOLD : blocks, e = blockIdx.y * 256 + threadIdx.x;
+    if (e > E) return;
+    int c = 0;
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) c += part_c[(long)b * (E + 1) + e];
+    to_c[(long)blockIdx.x * (E + 1) + e] = c;
+    if (e == E) return;
+    float s = 0.f;
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) s += part_p[(long)b * E + e];
+    to_p[(long)blockIdx.x * E + e] = s;
 }
 
 // Joins the parts: 1024 threads, the columns side by side and as many runs of parts as fit, each in part order.
@@ -163,7 +178,7 @@ __global__ __launch_bounds__(1024) void k_balance_join(const float *part_p, cons
     int c = 0;
     if (run < runs) {
         const int per = (blocks + runs - 1) / runs, b0 = run * per, b1 = b0 + per < blocks ? b0 + per : blocks;
-#pragma unroll 8
+#pragma unroll 16
         for (int b = b0; b < b1; ++b) { s += part_p[(long)b * E + e]; c += part_c[(long)b * (E + 1) + e]; }
     }
     int v = 0;
@@ -208,10 +223,10 @@ __global__ __launch_bounds__(WG) void k_balance_backward(const T *z, const unsig
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int i = 0; i < V; ++i) dot += f[j][i] * r.p[j][i];
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) dot += __shfl_xor(dot, o, UMR_WAVE);
+            for (int i = 0; i < V; ++i) dot = fmaf(f[j][i], r.x[j][i], dot);
+        dot = group_sum<LPR>(dot) * r.r;
         if (!here) continue;
+        const float up = scale * r.r;
         const bool valid = some && (!mask || mask[row]);
 #pragma unroll
         for (int j = 0; j < J; ++j)
@@ -220,7 +235,7 @@ __global__ __launch_bounds__(WG) void k_balance_backward(const T *z, const unsig
                 const int e0 = (j * LPR + s) * V + i0;
                 float v[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = valid ? scale * r.p[j][i0 + i] * (f[j][i0 + i] - dot) : 0.f;
+                for (int i = 0; i < 4; ++i) v[i] = valid ? up * r.x[j][i0 + i] * (f[j][i0 + i] - dot) : 0.f;
                 store4(dz + row * E + e0, E - e0, v);
             }
     }
@@ -242,9 +257,10 @@ __global__ __launch_bounds__(WG) void k_balance_backward(const T *z, const unsig
     }
 
 long rows_per_group(long T, int E) {
-    // a workgroup's 4 waves read about 1 KB each at a time; at most 512 workgroups, whose parts one workgroup joins
-    long rows = (T + 511) / 512, least = E > 0 ? 16384 / E : 1;
-    if (least < 16) least = 16;
+    // a workgroup's 16 waves take 16 KB of 16-bit or fp32 scores at a time, at least twice; at most 512 workgroups, whose parts one
+    // workgroup joins
+    long rows = (T + 511) / 512, least = 32768 / (4 * (E < 4 ? 4 : E));
+    if (least < 32) least = 32;
     return rows < least ? least : rows;
 }
 
@@ -254,6 +270,8 @@ bool balance_ok(long T, int E, int dtype) {
 
 long groups_of(long T, int E) { const long r = rows_per_group(T, E); return T > 0 ? (T + r - 1) / r : 1; }
 
+long folds_of(long groups) { return groups > 2 * FOLD ? (groups + FOLD - 1) / FOLD : 0; }
+
 }  // namespace
 
 extern "C" {
@@ -261,7 +279,7 @@ extern "C" {
 size_t umr_balance_workspace_bytes(long T, int E) {
     if (!balance_ok(T, E, UMR_F32)) return 0;
     const long g = groups_of(T, E);
-    return g > 1 ? (size_t)g * (2 * E + 1) * 4 : 0;
+    return g > 1 ? (size_t)(g + folds_of(g)) * (2 * E + 1) * 4 : 0;
 }
 
 int umr_balance_forward(const void *z, const long long *inds, const unsigned char *mask, float *loss, long long *counts, float *coef, long T, int E,
@@ -273,14 +291,24 @@ int umr_balance_forward(const void *z, const long long *inds, const unsigned cha
     int *pc = groups > 1 ? (int *)workspace + groups * E : nullptr;
     const hipStream_t st = (hipStream_t)stream;
 #define UMR_CALL(TT, LPR, J)                                                                                                               \
-    UMR_LAUNCH((k_balance_rows<TT, LPR, J>), (unsigned)groups, WG, 0, st, (const TT *)z, inds, mask, pp, pc, loss, counts, coef, T, E, k, rows);
+    UMR_LAUNCH((k_balance_rows<TT, LPR, J>), (unsigned)groups, ROWS_WG, 0, st, (const TT *)z, inds, mask, pp, pc, loss, counts, coef, T, E, k, rows);
     if (dtype == UMR_F32) UMR_BALANCE_SHAPES(float, E, UMR_CALL)
     else if (dtype == UMR_BF16) UMR_BALANCE_SHAPES(bf16_t, E, UMR_CALL)
     else UMR_BALANCE_SHAPES(f16_t, E, UMR_CALL)
 #undef UMR_CALL
     if (umr_launch_status() != UMR_OK) return UMR_ERR_LAUNCH;
     if (groups > 1) {
-        UMR_LAUNCH(k_balance_join, 1, 1024, 0, st, (const float *)pp, (const int *)pc, (int)groups, loss, counts, coef, E, k);
+        long parts = groups;
+        if (const long folds = folds_of(groups)) {
+            float *to_p = (float *)(pc + groups * (E + 1));
+            int *to_c = (int *)(to_p + folds * E);
+            UMR_LAUNCH(k_balance_fold, dim3((unsigned)folds, (unsigned)(E / 256 + 1)), 256, 0, st, (const float *)pp, (const int *)pc, (int)groups, to_p, to_c, E);
+            if (umr_launch_status() != UMR_OK) return UMR_ERR_LAUNCH;
+            pp = to_p;
+            pc = to_c;
+            parts = folds;
+        }
+        UMR_LAUNCH(k_balance_join, 1, 1024, 0, st, (const float *)pp, (const int *)pc, (int)parts, loss, counts, coef, E, k);
         return umr_launch_status();
     }
     return UMR_OK;
