@@ -71,6 +71,8 @@ def parse():
     ap.add_argument("--grad-sync", default="buckets", choices=["buckets", "ddp"],
                     help="N > 1: `buckets` = umr_amd.parallel.BucketedGradSync (64 MB buckets all-reduced from gradient hooks while "
                          "backward runs; capturable); `ddp` = torch DistributedDataParallel (eager only: implies --graph 0)")
+    ap.add_argument("--fused-fc", type=int, default=0, help="1: MeshNet's fully connected layers as umr_amd.functional.linear_act")
+    ap.add_argument("--balance-wt", type=float, default=0.0, help="--workload s2: weight of the balance loss over the camera hypotheses")
     ap.add_argument("--hot-path-sub", type=int, default=-1,
                     help="1: also time the render-and-compare step alone (the --model 0 --graph 1 measurement) in this process and "
                          "attach it as config.hot_path_images_per_s / hot_path_ms_per_step; default: on for the --gpus 1 train_s1 "

@@ -270,6 +270,126 @@ def test_a_routers_operators_together():
         # a factor of at most 2 in the 2-norm (softmax, silu and the products of unit variance here do not enlarge it), fp32 sums of
         # up to 1600 terms add 1600 u
         tol = 10 * C.half_step(dtype) + 1600 * C.U
-        assert abs(float(loss.detach()) - float(l64)) <= tol * float(l64)
+        assert abs(float(loss.detach()) - float(l64.detach())) <= tol * float(l64.detach())
         for a, c in zip(grads, g64):
             assert float((a.double() - c).norm()) <= tol * float(c.norm())
+
+
+# ---------------------------------------------------------------------------------------------- the framework's own paths
+def _through(layers, x, err):
+    """(value, bound) of linear layers [(weight, bias, slope or None)] in 64 bits: a layer adds (K + 3) u of its magnitudes (sum, bias,
+    rounding) and passes the incoming error through |W|; a LeakyReLU does not enlarge it"""
+    for w, b, slope in layers:
+        w, b = w.double(), b.double()
+        mag = x.abs() @ w.abs().t() + b.abs()
+        x, err = x @ w.t() + b, err @ w.abs().t() + (w.shape[1] + 3) * C.U * mag
+        if slope is not None:
+            x = torch.nn.functional.leaky_relu(x, slope)
+            err = err + C.U * x.abs()
+    return x, err
+
+
+def test_fused_and_folded_camera_predictor_against_64_bits():
+    """MultiCamPredictor in eval mode, its layers fused and its cameras folded into three products, against the unfused module in
+    64 bits: shared stack, then per camera three layers; the folded weights are each rounded once (u of their own magnitude)"""
+    from umr_amd import model as M
+    torch.manual_seed(3)
+    net = M.MultiCamPredictor(200, 8).to(DEV)
+    for m in net.modules():
+        if isinstance(m, torch.nn.Linear):
+            m.weight.data.normal_(0, 0.08)
+        if isinstance(m, torch.nn.BatchNorm1d):
+            m.running_mean.normal_(0, 0.3), m.running_var.uniform_(0.5, 2.0), m.weight.data.uniform_(0.5, 1.5), m.bias.data.normal_(0, 0.1)
+    net.eval()
+    folded = M.fold_for_inference(net)
+    feat = torch.randn(16, 200, device=DEV)
+    torch.manual_seed(0)
+    cam, inds, probs, cams, quats, logits = folded(feat, with_logits=True)
+    zero = torch.zeros(16, 200, device=DEV, dtype=torch.float64)
+    f, ferr = _through([(l[0].weight, l[0].bias, 0.1) for l in net.fc], feat.double(), zero)
+    got = M.fuse_linears(net).fc(feat)
+    assert bool(((got.double() - f).abs() <= ferr).all())
+    fc = folded.camera_predictor
+    for k, c in enumerate(net.camera_predictor):
+        h, err = f, ferr
+        with torch.no_grad():
+            for l in c.fc_layer:
+                s = l[1].weight.double() / torch.sqrt(l[1].running_var.double() + l[1].eps)
+                w, b = l[0].weight.double() * s[:, None], (l[0].bias.double() - l[1].running_mean.double()) * s + l[1].bias.double()
+                err = err + C.U * h.abs()                                    # (the folded weight's rounding)
+                h, err = _through([(w, b, 0.2)], h, err)
+            last = [(p.weight, p.bias) for p in (c.quat_predictor.pred_layer, c.prob_predictor, c.scale_predictor.pred_layer, c.trans_predictor.pred_layer)]
+            o, err = _through([(torch.cat([w for w, _ in last]), torch.cat([b for _, b in last]), None)], h, err)
+        assert bool(((logits[:, k].double() - o[:, 4]).abs() <= err[:, 4]).all())
+        assert bool(((cams[:, k, 1:3].double() - o[:, 6:8]).abs() <= err[:, 6:8]).all())
+        scale = torch.relu(c.scale_lr * o[:, 5] + c.scale_bias) + 1e-12
+        assert bool(((cams[:, k, 0].double() - scale).abs() <= err[:, 5] + 4 * C.U * scale.abs()).all())
+        q, n = o[:, :4], o[:, :4].norm(dim=1, keepdim=True)
+        # q / |q|: an error e of q moves it by at most 2 |e| / |q|; 8 roundings
+        assert bool(((quats[:, k].double() - q / n).abs() <= 2 * err[:, :4].norm(dim=1, keepdim=True) / n + 8 * C.U).all())
+    assert torch.equal(probs, torch.softmax(logits, 1)) and inds.shape == (16, 1)
+    assert fc.w2.shape == (8, 200, 200)
+
+
+def test_hypothesis_balance_loss_of_a_camera_predictor():
+    """loss_utils.hypothesis_balance_loss on what MeshNet gives it, gradients into every camera's layers"""
+    from umr_amd import loss_utils as LU, model as M
+    torch.manual_seed(3)
+    net = M.fuse_linears(M.MultiCamPredictor(200, 8)).to(DEV)
+    feat = torch.randn(16, 200, device=DEV)
+    out = net(feat, with_logits=True)
+    loss, counts = LU.hypothesis_balance_loss(out[5], out[1])
+    want, c64, d64, _ = C.balance64(out[5].detach(), out[1], None)
+    assert torch.equal(counts, c64) and int(counts.sum()) == 16
+    C.close(loss.detach(), want, 100 * C.U * want.abs(), "loss")
+    loss.backward()
+    for c in net.camera_predictor:
+        g = c.prob_predictor.weight.grad
+        assert g is not None and bool(torch.isfinite(g).all()) and float(g.abs().sum()) > 0
+
+
+def _training_step(workload):
+    import argparse
+    from umr_amd import model as M
+    from umr_amd.synthetic import make_s1_inputs
+    dev = torch.device(DEV)
+    args = argparse.Namespace(graph=1, batch=4, image_size=64 if workload == "s1" else 256, subdivide=2 if workload == "s1" else 3, epoch=0,
+                              share_mask_render=1, data_seed=100, fused_fc=1, balance_wt=0.5)
+    torch.manual_seed(77)
+    if workload == "s2":
+        return M, dev, M.build_training_step_s2(args, dev, 1)
+    tv, faces, _, _ = make_s1_inputs(4, 64, 2, seed=100, device=dev)
+    return M, dev, M.build_training_step(tv, faces, args, dev, 1)
+
+
+@pytest.mark.parametrize("workload", ["s1", "s2"])
+def test_training_step_with_fused_layers_and_the_balance_term(workload):
+    """the training steps with --fused-fc (and, for train_s2, the balance term): finite losses and gradients, and every layer's weights
+    move"""
+    M, dev, step = _training_step(workload)
+    net = step.model["net"]
+    assert sum(isinstance(m, M.Linear) for m in net.modules()) > 10
+    before = {n: p.detach().clone() for n, p in net.named_parameters() if p.requires_grad}
+    losses = [step() for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(bool(torch.isfinite(l)) for l in losses)
+    for n, p in net.named_parameters():
+        if p.requires_grad:
+            assert p.grad is not None and bool(torch.isfinite(p.grad).all()), n
+            # (train_s1's single camera multiplies its probability head by 0: its gradient is 0)
+            if n.endswith("weight") and not (workload == "s1" and "prob_predictor" in n):
+                assert not torch.equal(p, before[n]), n
+
+
+@pytest.mark.parametrize("workload", ["s1", "s2"])
+def test_training_step_with_fused_layers_replays_from_a_hip_graph(workload):
+    """the same step captured whole: a replay and an eager step from one saved state leave the same loss, moments and parameters, at the
+    bounds the step has without the fused layers"""
+    import os
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    from tests.test_gpu_round5 import replay_equals_eager
+    _, dev, step = _training_step(workload)
+    replay_equals_eager(step, dev, workload + " fused", bn_eval=True)

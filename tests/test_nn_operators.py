@@ -224,3 +224,52 @@ def test_operators_have_shapes_without_a_device():
     assert torch.autograd.grad(loss, z)[0].shape == z.shape
     with pytest.raises(RuntimeError, match="second time"):
         torch.autograd.grad(UF.linear_act(m(2, 6), w[0], activation="tanh").sum(), w, create_graph=True)
+
+
+# ---------------------------------------------------------------------------------------------- MeshNet's layers (host tensors: plain torch)
+def _tiny_net(seed=0, **kw):
+    from umr_amd import model as M
+    torch.manual_seed(seed)
+    opts = M.default_opts(multiple_cam_hypo=True, subdivide=1, **kw)
+    return M, M.MeshNet((64, 64), opts, nz_feat=opts.nz_feat)
+
+
+def test_fused_layers_keep_the_state_dict_and_the_values():
+    import copy
+    M, net = _tiny_net()
+    fused = M.fuse_linears(copy.deepcopy(net))
+    assert list(fused.state_dict()) == list(net.state_dict())
+    assert not any(type(m) is torch.nn.Linear for m in fused.modules()) and sum(isinstance(m, M.Linear) for m in fused.modules()) == \
+        sum(type(m) is torch.nn.Linear for m in net.modules())
+    # a LeakyReLU right behind a layer moved into it: the hypotheses' shared stack, the two latent heads; one behind a batch norm stayed
+    assert [l[0].activation for l in fused.cam_predictor.fc] == ["leaky_relu"] * 2 and fused.cam_predictor.fc[0][0].slope == pytest.approx(0.1)
+    assert fused.encoder.mean_fc[0].activation == "leaky_relu" and fused.encoder.enc_fc[0][0].activation == "none"
+    assert type(fused.encoder.enc_fc[0][2]) is torch.nn.LeakyReLU and type(fused.encoder.mean_fc[1]) is torch.nn.Identity
+    assert M.MeshNet((64, 64), M.default_opts(subdivide=1, fused_fc=True)).shape_predictor.pred_layer.__class__ is M.Linear
+    x = torch.randn(2, 3, 64, 64)
+    torch.manual_seed(5)
+    a = net(x)
+    torch.manual_seed(5)
+    b = fused(x)
+    assert list(a) == list(b) and all(torch.equal(a[k], b[k]) for k in a)
+    assert torch.equal(torch.softmax(a["cam_logits"], 1), a["cam_probs"])
+
+
+def test_folded_net_equals_the_net_in_eval_mode():
+    M, net = _tiny_net(1)
+    for k in range(3):                                                   # running statistics that are not the initial ones
+        net(torch.randn(4, 3, 64, 64))
+    net = net.double().eval()
+    folded = M.fold_for_inference(net)
+    assert not any(isinstance(m, torch.nn.BatchNorm1d) for m in folded.modules()) and not any(p.requires_grad for p in folded.parameters())
+    assert isinstance(folded.cam_predictor.camera_predictor, M.FoldedCameras) and not isinstance(net.cam_predictor.camera_predictor, M.FoldedCameras)
+    again = M.fold_for_inference(M.fuse_linears(net))                    # of a net whose layers were fused already
+    x = torch.randn(2, 3, 64, 64).double()
+    outs = []
+    for m in (net, folded, again):
+        torch.manual_seed(5)
+        outs.append(m(x))
+    for k in outs[0]:
+        for o in outs[1:]:       # in 64 bits: the same numbers in another order of operations (scale_bias and 1e-12 of the cameras are fp32 constants' sums)
+            assert float((outs[0][k].double() - o[k].double()).abs().max()) <= 1e-9 * max(1.0, float(outs[0][k].double().abs().max())), k
+

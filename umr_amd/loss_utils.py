@@ -40,6 +40,14 @@ def sym_reg(verts):
     return UF.abs_column_mean(verts, 1)
 
 
+def hypothesis_balance_loss(cam_logits, cam_sample_inds, mask=None):
+    """-> (loss, counts): how unevenly a batch uses its K camera hypotheses (not in the reference).  cam_logits [B,K]: the scores
+    before the softmax, cam_sample_inds [B,1] (or [B,k]): the hypotheses that were sampled, mask [B] bool: images that count.
+    K sum_k f_k P_k with f the share of samples and P the mean probability of hypothesis k: 1 when all are used alike, K when one
+    is; counts [K] int64 (umr_balance_*)."""
+    return UF.balance_loss(cam_logits, cam_sample_inds, mask)
+
+
 class TexCycle(nn.Module):
     """nnutils/loss_utils.py:152-182.  The per-sample torch.unique + host mask + H2D copy of the
     reference (:173-179) is one kernel (umr_visible_face_mask); id -1 still marks the last face."""

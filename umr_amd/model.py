@@ -27,7 +27,8 @@ def default_opts(**kw):
     o = dict(symmetric=True, symmetric_texture=True, multiple_cam_hypo=False, nz_feat=200, z_dim=350, num_hypo_cams=8,
              use_texture=True,
              tex_size=6, subdivide=3, batch_size=16, gpu_num=1, scale_lr_decay=0.05, scale_bias=1.0, pred_cam=True,
-             learning_rate=1e-4, beta1=0.9, grl_wt=0.2)
+             learning_rate=1e-4, beta1=0.9, grl_wt=0.2,
+             fused_fc=False)        # fully connected layers as functional.linear_act (fuse_linears); same parameters and keys
     o.update(kw)
     return SimpleNamespace(**o)
 
@@ -59,6 +60,78 @@ def fc_stack(nc_inp, nc_out, nlayers, use_bn=True):
     enc = nn.Sequential(*mods)
     net_init(enc)
     return enc
+
+
+def _linear_act(x, weight, bias, activation, slope):
+    """functional.linear_act on the GPU; on the CPU (tests of the DDP harness) plain torch, as Upsample2x."""
+    if x.is_cuda:
+        from .functional import linear_act
+        return linear_act(x, weight, bias, activation=activation, slope=slope)
+    y = F.linear(x, weight, bias)
+    return F.leaky_relu(y, slope) if activation == "leaky_relu" else y
+
+
+def _heads_linear_act(x, weight, bias, activation, slope):
+    """functional.heads_linear_act on the GPU, plain torch on the CPU: x [B, G, K], weight [G, N, K] -> [B, G, N]."""
+    if x.is_cuda:
+        from .functional import heads_linear_act
+        return heads_linear_act(x, weight, bias, activation=activation, slope=slope)
+    y = torch.matmul(x.transpose(0, 1), weight.transpose(1, 2)).transpose(0, 1) + bias
+    return F.leaky_relu(y, slope) if activation == "leaky_relu" else y
+
+
+class Linear(nn.Linear):
+    """nn.Linear (same parameters, same state_dict keys) with the LeakyReLU that follows it in the product's epilogue.  Made by
+    fuse_linears."""
+    activation, slope = "none", 0.0
+
+    def forward(self, x):
+        return _linear_act(x, self.weight, self.bias, self.activation, self.slope)
+
+
+def fuse_linears(net):
+    """Turn every nn.Linear of `net` into Linear, in place, and let it apply a LeakyReLU that directly follows it in a Sequential
+    (nn.Identity takes that place: module names, parameters and state_dict keys stay).  Returns net."""
+    for m in list(net.modules()):
+        kids = list(m._modules.items())
+        for k, (_, a) in enumerate(kids):
+            if not isinstance(a, nn.Linear) or getattr(a, "activation", "none") != "none":
+                continue
+            if type(a) is nn.Linear:
+                a.__class__ = Linear
+            if isinstance(m, nn.Sequential) and k + 1 < len(kids) and type(kids[k + 1][1]) is nn.LeakyReLU:
+                a.activation, a.slope = "leaky_relu", float(kids[k + 1][1].negative_slope)
+                m._modules[kids[k + 1][0]] = nn.Identity()
+    return net
+
+
+def _fold_batch_norm(lin, bn):
+    """(weight, bias) of the layer that equals bn(lin(x)) with bn's running statistics; formed in 64 bits."""
+    s = bn.weight.double() / torch.sqrt(bn.running_var.double() + bn.eps)
+    return (lin.weight.double() * s[:, None]).to(lin.weight.dtype), ((lin.bias.double() - bn.running_mean.double()) * s + bn.bias.double()).to(lin.bias.dtype)
+
+
+@torch.no_grad()
+def fold_for_inference(net):
+    """A copy of `net` (MeshNet or a part of it) for inference: eval mode, no gradients, every Linear + BatchNorm1d [+ LeakyReLU] of
+    a Sequential folded into one layer, and the cameras of a MultiCamPredictor as three layers for all of them at once (its first
+    layer is shared input: one product; the others one product a camera, in one launch).  The weights are laid out here, once."""
+    import copy
+    net = copy.deepcopy(net).eval()
+    for p in net.parameters():
+        p.requires_grad_(False)
+    for m in list(net.modules()):
+        kids = list(m._modules.items()) if isinstance(m, nn.Sequential) else []
+        for (_, a), (name, b) in zip(kids, kids[1:]):
+            if isinstance(a, nn.Linear) and getattr(a, "activation", "none") == "none" and type(b) is nn.BatchNorm1d:
+                w, bias = _fold_batch_norm(a, b)
+                a.weight.copy_(w)
+                a.bias.copy_(bias)
+                del m._modules[name]                      # (the LeakyReLU now follows the Linear)
+    for m in list(net.modules()):
+        if isinstance(m, MultiCamPredictor):
+            m.camera_predictor = FoldedCameras(m.camera_predictor)
+    return fuse_linears(net)
 
 
 class _ConvStagedBiasGrad(torch.autograd.Function):
@@ -284,6 +357,33 @@ class Camera(nn.Module):
         return torch.cat([quat, self.prob_predictor(f), scale, self.trans_predictor(f)], dim=1)
 
 
+class FoldedCameras(nn.Module):
+    """The K Camera heads of a MultiCamPredictor as three layers (fold_for_inference): [B, nz] -> [B, K, 8], what
+    torch.stack([camera(f) for camera in cameras], 1) gives."""
+
+    def __init__(self, cameras):
+        super().__init__()
+        cameras = list(cameras)
+        first, second = [c.fc_layer[0][0] for c in cameras], [c.fc_layer[1][0] for c in cameras]
+        last = [[c.quat_predictor.pred_layer, c.prob_predictor, c.scale_predictor.pred_layer, c.trans_predictor.pred_layer] for c in cameras]
+        self.register_buffer("w1", torch.cat([l.weight for l in first]))
+        self.register_buffer("b1", torch.cat([l.bias for l in first]))
+        self.register_buffer("w2", torch.stack([l.weight for l in second]))
+        self.register_buffer("b2", torch.stack([l.bias for l in second]))
+        self.register_buffer("w3", torch.stack([torch.cat([l.weight for l in ls]) for ls in last]))
+        self.register_buffer("b3", torch.stack([torch.cat([l.bias for l in ls]) for ls in last]))
+        self.register_buffer("scale_lr", torch.tensor([float(c.scale_lr) for c in cameras], device=self.w1.device)[:, None])
+        self.register_buffer("scale_bias", torch.tensor([float(c.scale_bias) for c in cameras], device=self.w1.device)[:, None])
+        self.slope = [float(c.fc_layer[i][1].negative_slope) for c in cameras[:1] for i in (0, 1)]
+
+    def forward(self, f):
+        h = _linear_act(f, self.w1, self.b1, "leaky_relu", self.slope[0]).unflatten(-1, self.w2.shape[::2])
+        h = _heads_linear_act(h, self.w2, self.b2, "leaky_relu", self.slope[1])
+        o = _heads_linear_act(h, self.w3, self.b3, "none", 0.0)
+        quat, prob, scale, trans = o[..., 0:4], o[..., 4:5], o[..., 5:6], o[..., 6:8]
+        return torch.cat([F.normalize(quat, dim=-1), prob, F.relu(self.scale_lr * scale + self.scale_bias) + 1e-12, trans], dim=-1)
+
+
 class MultiCamPredictor(nn.Module):
     """cub_mesh.py:303-362: K camera hypotheses + multinomial sampling."""
 
@@ -312,9 +412,14 @@ class MultiCamPredictor(nn.Module):
                          a1 * c2 - b1 * d2 + c1 * a2 + d1 * b2, a1 * d2 + b1 * c2 - c1 * b2 + d1 * a2))
         self.register_buffer("cam_biases", torch.tensor(bias, dtype=torch.float32))
 
-    def forward(self, feat):
+    def forward(self, feat, with_logits=False):
+        """-> (sampled camera [B,7], its index [B,1], probabilities [B,K], all cameras [B,K,7], quaternions [B,K,4]) and, if asked
+        for, the scores the probabilities are the softmax of [B,K]"""
         f = self.fc(feat)
-        cams = torch.stack([c(f) for c in self.camera_predictor], dim=1)      # [B,K,8]
+        if isinstance(self.camera_predictor, FoldedCameras):
+            cams = self.camera_predictor(f)
+        else:
+            cams = torch.stack([c(f) for c in self.camera_predictor], dim=1)      # [B,K,8]
         probs = F.softmax(cams[:, :, 4], dim=1)
         cam = torch.cat([cams[:, :, 5:6], cams[:, :, 6:8], cams[:, :, 0:4], probs.unsqueeze(-1)], dim=2)
         # per-rank RNG stream (:358-359).  torch.multinomial device-asserts on a non-finite probability and the assert takes the
@@ -322,7 +427,8 @@ class MultiCamPredictor(nn.Module):
         # non-finite rows are sampled uniformly (finite rows are untouched: nan_to_num is the identity on them)
         inds = torch.multinomial(torch.nan_to_num(probs.detach(), nan=1.0, posinf=1.0, neginf=0.0).clamp_min(1e-30), 1)
         sampled = torch.gather(cam, 1, inds.unsqueeze(-1).expand(-1, 1, 8)).squeeze(1)[:, 0:7]
-        return sampled, inds, cam[:, :, 7], cam[:, :, 0:7], cams[:, :, 0:4]
+        out = (sampled, inds, cam[:, :, 7], cam[:, :, 0:7], cams[:, :, 0:4])
+        return out + (cams[:, :, 4],) if with_logits else out
 
 
 class Discriminator(nn.Module):
@@ -409,13 +515,15 @@ class MeshNet(nn.Module):
         self.texture_predictor = TexturePredictorUV(nz_feat, num_faces, T, img_H=img_H, img_W=2 * img_H,
                                                     num_sym_faces=self.num_sym_faces if self.symmetric_texture else 0)
         net_init(self.texture_predictor)
+        if getattr(opts, "fused_fc", False):
+            fuse_linears(self)
 
     def forward(self, img=None):
         out = {}
         img_feat, noise, mean, logvar = self.encoder(img)
         out['delta_v'] = self.shape_predictor(noise).view(img.size(0), -1, 3)
         if self.opts.multiple_cam_hypo:
-            cam, inds, probs, all_cams, quats = self.cam_predictor(img_feat)
+            cam, inds, probs, all_cams, quats, out['cam_logits'] = self.cam_predictor(img_feat, with_logits=True)
             out['cam_hypotheses'], out['base_quats'] = all_cams, quats[:, 0]
         else:
             c = self.cam_predictor(img_feat)
@@ -458,7 +566,7 @@ def build_training_step(tv, faces, args, dev, world):
     from .image_utils import compute_dt_barrier
     from .synthetic import make_s1_inputs
     from .train_step import RenderCompareS1
-    opts = default_opts(subdivide=args.subdivide, batch_size=args.batch)
+    opts = default_opts(subdivide=args.subdivide, batch_size=args.batch, fused_fc=bool(getattr(args, "fused_fc", 0)))
     net = MeshNet((args.image_size, args.image_size), opts, nz_feat=opts.nz_feat).to(dev)
     disc = Discriminator(opts.grl_wt, img_size=args.image_size).to(dev)
     model = nn.ModuleDict(dict(net=net, disc=disc))
@@ -521,8 +629,8 @@ def build_training_step_s2(args, dev, world):
     backward with DDP all-reduce -> Adam.  SCOPS data being absent, part labels / points are synthetic."""
     from .image_utils import compute_dt_barrier
     from .synthetic import make_s2_inputs
-    from .train_step import RenderCompareS2
-    opts = default_opts(subdivide=args.subdivide, batch_size=args.batch, multiple_cam_hypo=True)
+    from .train_step import RenderCompareS2, S2Weights
+    opts = default_opts(subdivide=args.subdivide, batch_size=args.batch, multiple_cam_hypo=True, fused_fc=bool(getattr(args, "fused_fc", 0)))
     net = MeshNet((args.image_size, args.image_size), opts, nz_feat=opts.nz_feat).to(dev)
     disc = Discriminator(opts.grl_wt, in_dim=3, img_size=args.image_size).to(dev)     # train_s2.py:91-93: rgb input
     model = nn.ModuleDict(dict(net=net, disc=disc))
@@ -530,8 +638,10 @@ def build_training_step_s2(args, dev, world):
     rank = torch.distributed.get_rank() if (world > 1 and torch.distributed.is_initialized()) else 0
     _, _, _, batch, ex = make_s2_inputs(args.batch, opts.num_hypo_cams, args.image_size, args.subdivide,
                                         seed=getattr(args, "data_seed", 100) + rank, device=dev)
+    weights = S2Weights()
+    weights.balance_loss_wt = float(getattr(args, "balance_wt", 0.0))
     rc = RenderCompareS2(net.get_mean_shape().detach(), net.faces, ex["part_vertex_ids"], ex["uv_img"],
-                         net.uv_sampler, args.image_size, opts.num_hypo_cams, texture_loss_type="perceptual",
+                         net.uv_sampler, args.image_size, opts.num_hypo_cams, weights=weights, texture_loss_type="perceptual",
                          discriminator=ddp_disc, tex_size=opts.tex_size,
                          num_sym_faces=net.texture_predictor.num_sym_faces,
                          share_mask_render=bool(getattr(args, "share_mask_render", 1))).to(dev)      # train_s2.py:154-161

@@ -192,6 +192,7 @@ class S2Weights:
     prob_loss_wt = 5.0
     vertex_loss_wt = 10.0
     deform_reg_wt = 1.0
+    balance_loss_wt = 0.0         # not in the reference: > 0 adds the balance loss over the K hypotheses (needs outputs["cam_logits"])
 
 
 class RenderCompareS2(nn.Module):
@@ -199,7 +200,8 @@ class RenderCompareS2(nn.Module):
     21 backwards per image: MultiMaskLoss (8), MultiTextureLoss (8 + 1 hard), GAN view (1), part matching (4),
     chamfer vertex-part correspondence.
 
-    outputs: pred_vs [B,V,3], delta_v, mean_shape [V,3], cam [B,7], cam_hypotheses [B,K,7], cam_probs [B,K], tex_flow
+    outputs: pred_vs [B,V,3], delta_v, mean_shape [V,3], cam [B,7], cam_hypotheses [B,K,7], cam_probs [B,K], tex_flow; with
+             weights.balance_loss_wt also cam_logits [B,K] and cam_sample_inds [B,1]
     batch:   imgs, masks, dts_barrier, gan_angles [B], part_segs [B,5,H,H], random_imgs [B,3,H,H] (previous step's
              masked images, :268), head/belly/back/neck_points [B,n,2]
     """
@@ -266,7 +268,10 @@ class RenderCompareS2(nn.Module):
         corr = self.corr_loss_fn(rep(batch["head_points"]), rep(batch["belly_points"]), rep(batch["back_points"]),
                                  rep(batch["neck_points"]), rep(mean_shape), cams_all_hypo.reshape(-1, 7), avg=False)
         t["corr"] = (corr.view(B, K) * cam_probs.detach()).sum(dim=1).mean()                        # :313-314
-        total = weighted_total(self, t, [
+        balance_wt = getattr(w, "balance_loss_wt", 0.0)
+        if balance_wt:      # keeps the sampling from settling on a few of the hypotheses; cam_div (:222) looks at one image at a time
+            t["balance"], _ = loss_utils.hypothesis_balance_loss(outputs["cam_logits"], outputs["cam_sample_inds"])
+        total = weighted_total(self, t, ([("balance", balance_wt)] if balance_wt else []) + [
             ("mask", w.mask_loss_wt), ("triangle", w.triangle_reg_wt), ("flatten", w.flatten_reg_wt),
             ("deform", w.deform_reg_wt), ("tex", w.tex_loss_wt), ("tex_dt", w.tex_dt_loss_wt),
             ("tex_cycle", w.tex_cycle_loss_wt), ("gan", w.gan_loss_wt), ("cam_div", w.ent_loss_wt),
