@@ -34,9 +34,8 @@ namespace {
 
 // Record layout (floats) written by k_face_setup: 256 bytes per face.
 //   [0,32)  wave-uniform part, fetched with 2 x s_load_dwordx16 into SGPRs.  Quantities that enter the geometry as 2-vectors
-//           sit in EVEN-ALIGNED PAIRS so that they are operands of packed fp32 instructions straight from the scalar file:
-//           on gfx950 a v_mul_f32 with an SGPR source issues in 4.2 cycles per wave, a v_pk_mul_f32 with an SGPR PAIR source in
-//           4.3 -- two products for the price of one (tools/ubench/valu_ubench2.hip, profiles/r04_valu_ubench2.log)
+//           sit in EVEN-ALIGNED PAIRS (laid out so when they were operands of packed fp32 instructions; the build makes two
+//           scalar instructions of such a pair now, see FLAGS in umr_amd/build.py -- same bits, same step time)
 //   [32,36) reciprocal depths (third scalar load, only in the kernels that interpolate depth)
 //   [40,64) three 32-byte edge blocks {a0, a1, a2, a[v1], den, RN(1/den), -, -}; a lane reads ONLY the block
 //           of its nearest edge (per-lane address, 2 x global_load_dwordx4, L1-resident)
@@ -47,7 +46,7 @@ enum { R_XLO = 0, R_XHI = 1, R_YLO = 2, R_YHI = 3,
        R_FLAGS = 14,              // bits 0-1 obtuse corner + 1 | 2 slow division | 3 depth always in range | 4 ill-conditioned / thin
                                   // | 5 front-facing
        R_CULL = 15,               // how far beyond sqrt(threshold) the reference still includes pixels (tile_may_hit)
-       // inverse barycentric matrix, rows 0 and 1 interleaved: (inv0, inv3) (inv1, inv4) (inv2, inv5) -> (w0, w1) in three packed ops
+       // inverse barycentric matrix, rows 0 and 1 interleaved: (inv0, inv3) (inv1, inv4) (inv2, inv5) -> (w0, w1) in three 2-vector ops
        R_I0 = 16, R_I3 = 17, R_I1 = 18, R_I4 = 19, R_I2 = 20, R_I5 = 21, R_I6 = 22, R_I7 = 23, R_I8 = 24,
        R_K2 = 25, R_K0 = 26, R_K1 = 27,                                  // squared heights; (K0, K1) is a pair
        R_Z0 = 28, R_Z1 = 29, R_Z2 = 30,
@@ -343,7 +342,7 @@ struct Face {  // wave-uniform: 32 (+ 4) SGPRs + the record's address
         else if constexpr (I < 32) return qb[I - 16];
         else return qc[I - 32];
     }
-    // an even-aligned pair (I, I + 1) of the record as a 2-vector: an SGPR pair, i.e. one source operand of a packed fp32 op
+    // an even-aligned pair (I, I + 1) of the record as a 2-vector: an SGPR pair
     template <int I> __device__ __forceinline__ v2f g2() const {
         static_assert((I & 1) == 0 && I < 32, "pairs are even-aligned and live in the first 32 floats");
         if constexpr (I < 16) return __builtin_shufflevector(qa, qa, I, I + 1);
@@ -351,7 +350,7 @@ struct Face {  // wave-uniform: 32 (+ 4) SGPRs + the record's address
     }
     template <int I> __device__ __forceinline__ float inv() const { return g<r_inv(I)>(); }   // the reference's face_inv[I]
     // barycentrics (:25-29) and the offset sum (:95-96, :148-149) in the reference's operation order, rounded once per
-    // operation; here two rows / both components at a time as packed ops on SGPR pairs
+    // operation; here two rows / both components at a time
     __device__ __forceinline__ void bary(float &w0, float &w1, float &w2, float xp, float yp) const {
         const v2f w01 = (g2<R_I0>() * splat2(xp) + g2<R_I1>() * splat2(yp)) + g2<R_I2>();
         w0 = w01.x; w1 = w01.y;
@@ -373,7 +372,7 @@ struct Face {  // wave-uniform: 32 (+ 4) SGPRs + the record's address
 // + 15 VGPRs per lane, filled once per face by the face-major backward (a wave owns one face for all its visits): the operands
 // of the barycentric rows and of the offset sums as VGPR copies.  On gfx950 a VALU instruction with an SGPR source issues at half
 // the rate of the same instruction on VGPRs (v_mul_f32 2.6 vs 4.2 cycles per wave-instruction); plain full-rate ops on these copies
-// measured faster in the backward than packed ops on them (dependent packed ops want a wait state in between).
+// measured faster in the backward.
 struct FaceV : Face {
     float vinv[9], vxy[6];
     __device__ __forceinline__ void bary(float &w0, float &w1, float &w2, float xp, float yp) const {
@@ -441,9 +440,8 @@ __device__ __forceinline__ float fmed3_(float a, float b, float c) {   // v_med3
 // bbox reject (:355), barycentric (:25-29), euclidean distance (:63-152), threshold reject (:382),
 // sigmoid (:383).  Returns false when the reference would `continue` before touching the pixel.
 //
-// Arithmetic: every product and sum is the reference's, in the reference's order, rounded once each (-ffp-contract=off); where
-// two of them are independent and their scalar operands sit in an aligned pair of the record they are issued as ONE packed
-// instruction (v_pk_mul_f32 / v_pk_add_f32 are per-component IEEE operations: the bits are those of the two scalar ops).
+// Arithmetic: every product and sum is the reference's, in the reference's order, rounded once each (-ffp-contract=off); two
+// independent ones whose scalar operands sit in an aligned pair of the record are written as one 2-vector operation.
 //
 // REGION (compile time; raster kernels pick it per visit with one wave vote, see eval_pair_voted):
 //   0  lanes on both sides of the boundary: everything below
