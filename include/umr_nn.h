@@ -6,7 +6,8 @@
  *   - `dtype` names the type of every tensor passed as void*: UMR_F32, UMR_BF16 or UMR_F16; all sums are fp32
  *   - a matrix operand is described by its element strides (row, head); its last dimension has stride 1.  Strides of 0 are
  *     allowed in operands that are read (a broadcast), outputs are dense
- *   - sizes may be 0 (an empty product is 0); M, N, K < 2^31 - 256, G < 65536, M * G * max(N, K) < 2^46
+ *   - outputs and workspaces overlap nothing else of the call (parts of a result may be written twice, with the same bits)
+ *   - sizes may be 0 (an empty product is 0); M, N, K < 2^27, G < 65536, M * G * max(N, K) < 2^46
  */
 #ifndef UMR_NN_H
 #define UMR_NN_H
@@ -58,7 +59,7 @@ size_t umr_linear_grad_weight_workspace_bytes(long M, long N, long K, int G, int
 int umr_linear_grad_weight(const void *dz, long dz_row, long dz_head, const void *x, long x_row, long x_head, void *dw, long M, long N,
                            long K, int G, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
-/* Balance loss over E choices (1 <= E <= UMR_BALANCE_MAX_CHOICES).  Rows t < T with scores z[t,:] (T x E, dense), of which k
+/* Balance loss over E choices (1 <= E <= UMR_BALANCE_MAX_CHOICES).  Rows t < T with scores z[t,:] (T x E, dense), T * k < 2^31, of which k
  * choices inds[t,:] (T x k, dense, k >= 1) were taken:
  *     p[t,:] = softmax(z[t,:])        over the valid rows, n of them:
  *     counts[e] = #{(t,j): inds[t,j] = e},   f_e = counts[e] / (n k),   P_e = mean_t p[t,e],      loss = E sum_e f_e P_e

@@ -28,6 +28,14 @@ def test_linear_against_64_bits(M, G, N, K, pad, dtype):
     C.check_linear(_lib(), M, G, N, K, dtype, "silu", device=DEV, pad=pad)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_linear_largest_tiles_against_64_bits(dtype):
+    """enough 16-bit results for the 256 x 256 tiles, with tiles that overlap in both directions and a cut last step, in each product"""
+    C.check_linear(_lib(), 4100, 1, 4099, 203, dtype, "gelu", device=DEV, pad=1, parts=("forward",))
+    C.check_linear(_lib(), 4100, 1, 77, 4099, dtype, "none", device=DEV, parts=("input",))
+    C.check_linear(_lib(), 77, 1, 4100, 4099, dtype, "none", device=DEV, parts=("weight",))
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("act", list(H.ACT))
 def test_linear_activations(act, dtype):
@@ -177,6 +185,57 @@ def test_offsets_beyond_32_bits():
     assert abs(float(loss.detach()) - 1.0) < 1e-4
     dz, = torch.autograd.grad(loss, z, torch.tensor(float(T), device=DEV))
     assert float(dz[-1].abs().sum()) < 1e-6 and bool((dz[-2] == dz[0]).all()) and float(dz[0, 0]) > 0
+
+
+def test_rows_far_apart_in_many_row_products():
+    """rows of 2^22 elements and more in memory, more than 64 of them: the tiled kernels' 64-bit loads, for each operand of each product
+    and each type; the same bits as from contiguous copies"""
+    from umr_amd import functional as UF
+    g = torch.Generator(device=DEV).manual_seed(3)
+    for dtype in (torch.float32, torch.bfloat16):
+        big = torch.zeros(70, (1 << 22) + 3, device=DEV, dtype=dtype)
+        for K in (40, 3, 131):
+            x = big[:, 5:5 + K]
+            x.copy_(torch.randn(70, K, device=DEV, generator=g))
+            near = x.contiguous()
+            w = torch.randn(90, K, device=DEV, generator=g).to(dtype)
+            gy = torch.randn(70, 90, device=DEV, generator=g).to(dtype)
+            gy2 = torch.randn(90, 70, device=DEV, generator=g).to(dtype)
+            far_gy = big[:, 1000:1090]
+            far_gy.copy_(gy)
+            for a, b in ((x, near),):
+                la, lb, wl = a.detach().requires_grad_(True), b.detach().requires_grad_(True), w.clone().requires_grad_(True)
+                ya, yb = UF.linear_act(la, wl), UF.linear_act(lb, wl)            # x far: the fast Q operand, in dw the slow P one
+                assert torch.equal(ya, yb)
+                for u, v in zip(torch.autograd.grad(ya, [la, wl], far_gy), torch.autograd.grad(yb, [lb, wl], gy)):   # dz far: fast and slow Q
+                    assert torch.equal(u, v)
+                ya, yb = UF.linear_act(wl, la), UF.linear_act(wl, lb)            # the weight far: the fast P operand, in dx the slow one
+                assert torch.equal(ya, yb)
+                for u, v in zip(torch.autograd.grad(ya, [wl, la], gy2), torch.autograd.grad(yb, [wl, lb], gy2)):
+                    assert torch.equal(u, v)
+
+
+@pytest.mark.parametrize("want", ["x", "w", "b", "r", "xb", "wr", "br", "xwr"])
+@pytest.mark.parametrize("bias", [True, False])
+def test_gradients_of_some_inputs_only(want, bias):
+    """any subset of the inputs may want a gradient, with and without a bias: each gets what it gets when all do, nothing else does"""
+    from umr_amd import functional as UF
+    x, w, b, r, gy = C.inputs(20, 2, 9, 7, torch.float32, DEV)
+    for res in (r, r[0]):
+        every = {k: v.detach().clone().requires_grad_(True) for k, v in dict(x=x, w=w, b=b, r=res).items()}
+        call = lambda t: UF.heads_linear_act(t["x"], t["w"], t["b"] if bias else None, residual=t["r"], activation="gelu")
+        names = [n for n in "xwbr" if bias or n != "b"]
+        full = dict(zip(names, torch.autograd.grad(call(every), [every[n] for n in names], gy)))
+        some = {k: v.detach().clone().requires_grad_(k in want) for k, v in every.items()}
+        picked = [n for n in want if n in names]
+        if not picked:
+            assert not call(some).requires_grad
+            continue
+        call(some).backward(gy)
+        for n in "xwbr":
+            assert (some[n].grad is not None) == (n in picked), n
+            if n in picked:
+                assert torch.equal(some[n].grad, full[n]), n
 
 
 def _capture(fn):

@@ -153,7 +153,7 @@ def test_c_abi_refusals():
         return L.umr_linear_forward(x, strides[0], strides[1], w, 4, 16, None, None, 0, 0, y, None, M, N, K, G, dtype, act, slope, ws, n, None)
     for kw in (dict(M=-1), dict(N=-1), dict(K=-1), dict(G=0), dict(G=65536), dict(dtype=3), dict(dtype=-1), dict(act=6), dict(act=-1),
                dict(act=2, slope=-0.1), dict(act=2, slope=float("nan")), dict(x=None), dict(w=None), dict(y=None), dict(strides=(-1, 0)),
-               dict(M=2 ** 31), dict(M=2 ** 30, G=60000)):
+               dict(M=2 ** 27), dict(N=2 ** 31), dict(M=2 ** 26, G=60000, N=2 ** 20)):
         assert forward(**kw) == -1, kw
     assert forward(M=0) == 0 and forward(N=0) == 0                          # nothing to do, nothing enqueued
     need = L.umr_linear_forward_workspace_bytes(16, 8, 8192, 1, 0)

@@ -10,7 +10,7 @@ Plan plan(int kind, long nq, long np, long nc, int G, int dtype) {
     Plan pl;
     const int es = dtype == UMR_F32 ? 4 : 2;
     pl.few = kind != GRAD_WEIGHT && nq <= 64;
-    pl.outer = kind == GRAD_WEIGHT && nc <= 64 && np >= 64 && nq >= 64;
+    pl.outer = kind == GRAD_WEIGHT && nc <= 64 && np >= 64 && nq >= 64 && ceil_div(nq, 64) <= 65535;
     pl.tile = 0;
     long groups, step;
     if (pl.few) {
@@ -40,8 +40,8 @@ Plan plan(int kind, long nq, long np, long nc, int G, int dtype) {
 size_t plan_bytes(const Plan &pl, long nq, long np, int G) { return pl.S > 1 ? (size_t)pl.S * G * nq * np * sizeof(float) : 0; }
 
 bool sizes_ok(long M, long N, long K, int G, int dtype) {
-    const long lim = 0x7fffffffL - 256;
-    if (M < 0 || N < 0 || K < 0 || G < 1 || G > 65535 || M > lim || N > lim || K > lim) return false;
+    const long lim = 1L << 27;                                // (a launch has at most 2^32 threads)
+    if (M < 0 || N < 0 || K < 0 || G < 1 || G > 65535 || M >= lim || N >= lim || K >= lim) return false;
     if (dtype != UMR_F32 && dtype != UMR_BF16 && dtype != UMR_F16) return false;
     const long wide = N > K ? N : K;
     return (double)M * G * wide < 7e13 && (double)G * N * K < 7e13;

@@ -809,7 +809,6 @@ template <class T> int run_product(int kind, const Plan &pl, Product pr, Epilogu
     int rc;
     if (pl.outer) {
         const dim3 grid((unsigned)ceil_div(pr.np, 256), (unsigned)ceil_div(pr.nq, 64), pr.G);
-        if (ceil_div(pr.nq, 64) > 65535) return UMR_ERR_ARG;
         const bool stream = (double)pr.nq * pr.np * pr.G * sizeof(T) >= 64e6;
         if (stream) UMR_LAUNCH((k_linear_outer<T, true>), grid, 256, 0, st, pr, (T *)e.out, e.o_row, e.o_head);
         else UMR_LAUNCH((k_linear_outer<T, false>), grid, 256, 0, st, pr, (T *)e.out, e.o_row, e.o_head);

@@ -772,7 +772,8 @@ def linear_act(x, weight, bias=None, residual=None, activation="none", slope=0.0
     float32, bfloat16 or float16, one type for all; sums are fp32 and a result is rounded once.  Any strides: rows that are
     contiguous are read in place, whatever lies between them.  Gradients to x, weight, bias and residual (in 16 bits the gradient of the
     pre-activation is rounded to 16 bits, as the operands of the matrix unit are); at a kink the derivative is the negative
-    side's.  Not differentiable twice.  The same inputs give the same bits in every call."""
+    side's.  Not differentiable twice.  The same inputs give the same bits in every call.
+    Fewer than 2^27 rows, columns and inputs; tensors on the current device, work on its current stream."""
     op, _, table = _nn_ops(x, weight, bias, residual)
     if weight.dim() != 2:
         raise RuntimeError("umr_amd: linear_act: weight must be [N, K], got %s" % list(weight.shape))
