@@ -19,15 +19,29 @@ template <class T, int LPR, int J> struct Row {          // one row's pieces in 
     static constexpr int V = 16 / (int)sizeof(T);
     float x[J][V], r;                                    // softmax = x r
 
-    // false: nothing to choose from (every score -inf)
-    __device__ __forceinline__ bool softmax(const T *z, int E, int s) {
+    // E a multiple of V (uniform): whole pieces, without the branches of a cut one
+    __device__ __forceinline__ void load(const T *z, int E, int s) {
+        if (E % V == 0) {
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int e0 = (j * LPR + s) * V;
-            const u32x4 v = load16B_n(z + e0, E - e0);
+            for (int j = 0; j < J; ++j) {
+                const int e0 = (j * LPR + s) * V;
+                const u32x4 v = load16B(z + (e0 < E ? e0 : 0));
 #pragma unroll
-            for (int i = 0; i < V; ++i) x[j][i] = e0 + i < E ? elem_of<T>(v, i) : -INFINITY;
+                for (int i = 0; i < V; ++i) x[j][i] = e0 < E ? elem_of<T>(v, i) : -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int e0 = (j * LPR + s) * V;
+                const u32x4 v = load16B_n(z + e0, E - e0);
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[j][i] = e0 + i < E ? elem_of<T>(v, i) : -INFINITY;
+            }
         }
+    }
+
+    // false: nothing to choose from (every score -inf)
+    __device__ __forceinline__ bool softmax() {
         float m = -INFINITY;                             // (a NaN is left out; it comes back through the exponentials)
 #pragma unroll
         for (int j = 0; j < J; ++j)
@@ -105,14 +119,18 @@ __global__ __launch_bounds__(ROWS_WG) void k_balance_rows(const T *z, const long
         const bool here = row < r1;
         const long safe = here ? row : r1 - 1;
         Row<T, LPR, J> r;
-        const bool some = r.softmax(z + safe * E, E, s);
-        if (!here || !some || (mask && !mask[row])) continue;
+        r.load(z + safe * E, E, s);
+        const long long chosen = s < k ? inds[safe * k + s] : -1;                // (on its way while the softmax is made)
+        const bool counts_here = here && (!mask || mask[safe]);
+        const bool some = r.softmax();
+        if (!counts_here || !some) continue;
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[j][i] = fmaf(r.x[j][i], r.r, acc[j][i]);
         if (s == 0) atomicAdd(&hist[W], 1);
-        for (int i = s; i < k; i += LPR) {
+        if (chosen >= 0 && chosen < E) atomicAdd(&hist[(int)chosen], 1);
+        for (int i = s + LPR; i < k; i += LPR) {
             const long long e = inds[row * k + i];
             if (e >= 0 && e < E) atomicAdd(&hist[(int)e], 1);
         }
@@ -200,7 +218,8 @@ __global__ __launch_bounds__(1024) void k_balance_join(const float *part_p, cons
 }
 
 template <class T, int LPR, int J>
-__global__ __launch_bounds__(WG) void k_balance_backward(const T *z, const unsigned char *mask, const float *coef, const float *grad, T *dz,
+__global__ __launch_bounds__(WG) void k_balance_backward(const T *__restrict__ z, const unsigned char *__restrict__ mask, const float *__restrict__ coef,
+                                                         const float *__restrict__ grad, T *__restrict__ dz,
                                                          long T_rows, int E) {
     constexpr int V = 16 / (int)sizeof(T), RPW = 64 / LPR;
     const int t = threadIdx.x, lane = t & 63, s = lane % LPR, sub = lane / LPR;
@@ -218,7 +237,8 @@ __global__ __launch_bounds__(WG) void k_balance_backward(const T *z, const unsig
         const long row = b + sub;
         const bool here = row < T_rows;
         Row<T, LPR, J> r;
-        const bool some = r.softmax(z + (here ? row : T_rows - 1) * E, E, s);
+        r.load(z + (here ? row : T_rows - 1) * E, E, s);
+        const bool some = r.softmax();
         float dot = 0.f;
 #pragma unroll
         for (int j = 0; j < J; ++j)

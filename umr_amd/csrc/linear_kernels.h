@@ -717,42 +717,65 @@ template <class T, bool STREAM> __global__ __launch_bounds__(256) void k_linear_
 }
 
 // ------------------------------------------------------------------------------------------------ act' and the sums over the rows
+template <int N> struct Count { static constexpr int value = N; };
+
 // One pass over gy and z.  A wave takes 256 columns (4 a lane) of the rows r0 + wave, r0 + wave + 4, ...; sums meet in LDS, and
-// over the row blocks in k_linear_colsum, both in a fixed order.
+// over the row blocks in k_linear_colsum, both in a fixed order.  The lanes at the right edge take the last 4 columns, some of them
+// twice, so that every load is 4 wide and none is behind a branch.
 template <class T>
-__global__ __launch_bounds__(256) void k_linear_act_grad(const T *gy, long g_row, long g_head, const void *z, T *dz, T *db, T *dr, float *part,
+__global__ __launch_bounds__(256) void k_linear_act_grad(const T *__restrict__ gy, long g_row, long g_head, const void *__restrict__ z, T *__restrict__ dz, T *db, T *dr, float *part,
                                                          long M, long N, int G, long rows, int act, float slope) {
     __shared__ __attribute__((aligned(16))) float red[2][4][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = blockIdx.z;
-    const long n = (long)blockIdx.x * 256 + lane * 4, left = N - n;
+    const long first = (long)blockIdx.x * 256, want = first + lane * 4;
+    const long n = want + 4 <= N || N < 4 ? want : N - 4, left = N - n;
     const long r0 = (long)blockIdx.y * rows, r1 = r0 + rows < M ? r0 + rows : M;
     float sz[4] = {0.f, 0.f, 0.f, 0.f}, sg[4] = {0.f, 0.f, 0.f, 0.f};
-    if (left > 0) {
-#pragma unroll 4
-        for (long m = r0 + wave; m < r1; m += 4) {
-            float gv[4], zv[4];
-            load4(gy + m * g_row + g * g_head + n, left, gv);
+    auto add = [&](auto count, long m, long wide) {           // rows m, m + 4, ..: every load before the first use
+        constexpr int B = decltype(count)::value;
+        float gv[B][4], zv[B][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sg[i] += gv[i];
+        for (int k = 0; k < B; ++k) load4(gy + (m + 4 * k) * g_row + g * g_head + n, wide, gv[k]);
+        if (dz) {
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                const long o = ((m + 4 * k) * G + g) * N + n;
+                if (kinked(act)) load4((const T *)z + o, wide, zv[k]);
+                else load4((const float *)z + o, wide, zv[k]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sg[i] += gv[k][i];
             if (dz) {
-                const long o = (m * G + g) * N + n;
-                if (kinked(act)) load4((const T *)z + o, left, zv);
-                else load4((const float *)z + o, left, zv);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) gv[i] *= act_slope<sizeof(T) == 4>(zv[i], act, slope);
+                for (int i = 0; i < 4; ++i) gv[k][i] *= act_slope<sizeof(T) == 4>(zv[k][i], act, slope);
                 // dz in the operator's own type: the operand of both gradient products (16-bit matrix instructions take 16 bits)
-                store4(dz + o, left, gv);
+                store4(dz + ((m + 4 * k) * G + g) * N + n, wide, gv[k]);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sz[i] += gv[i];
+            for (int i = 0; i < 4; ++i) sz[i] += gv[k][i];
         }
+    };
+    if (N >= 4) {                                             // (uniform)
+        if (want < N) {
+            long m = r0 + wave;
+            for (; m + 12 < r1; m += 16) add(Count<4>{}, m, 4);
+            for (; m < r1; m += 4) add(Count<1>{}, m, 4);
+        }
+    } else if (left > 0) {
+        for (long m = r0 + wave; m < r1; m += 4) add(Count<1>{}, m, left);
     }
     if (!db && !dr) return;                                   // (uniform)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { red[0][wave][lane * 4 + i] = sz[i]; red[1][wave][lane * 4 + i] = sg[i]; }
+    for (int i = 0; i < 4; ++i) {
+        const long k = n + i - first;                         // its column of this workgroup (the edge lane's first may be another's)
+        if (want < N && k >= 0 && k < 256) { red[0][wave][k] = sz[i]; red[1][wave][k] = sg[i]; }
+    }
     __syncthreads();
     const int i = threadIdx.x;
-    const long col = (long)blockIdx.x * 256 + i;
+    const long col = first + i;
     if (col >= N) return;
     const float a = ((red[0][0][i] + red[0][1][i]) + red[0][2][i]) + red[0][3][i];
     const float b = ((red[1][0][i] + red[1][1][i]) + red[1][2][i]) + red[1][3][i];
@@ -820,7 +843,6 @@ template <class T> int run_product(int kind, const Plan &pl, Product pr, Epilogu
         const bool near = pr.P.row < NEAR && pr.Q.row < NEAR && pr.np >= 256 && pr.nq >= 256 && pr.nc >= 8;
         if (pl.tile == T256x256 && !near) rc = launch_tile<T, 2, 2, 2, 2>(kind, pr, first, st);
         else if (pl.tile == T64x64) rc = launch_tile<T, 2, 2, 1, 1>(kind, pr, first, st);
-        else if (pl.tile == T128x64) rc = launch_tile<T, 2, 2, 2, 1>(kind, pr, first, st);
         else if (pl.tile == T128x128) rc = launch_tile<T, 2, 2, 2, 2>(kind, pr, first, st);
         else if constexpr (sizeof(T) == 2) rc = launch_tile<T, 2, 4, 4, 2>(kind, pr, first, st);
     }

@@ -33,8 +33,8 @@ inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
 constexpr int FEW_WAVES = 8;          // waves of a workgroup of the kernels for few rows
 
-enum Tile { T64x64, T128x64, T128x128, T256x256 };
-constexpr int TILE_Q[] = {64, 128, 128, 256}, TILE_P[] = {64, 64, 128, 256};
+enum Tile { T64x64, T128x128, T256x256 };
+constexpr int TILE[] = {64, 128, 256};
 
 struct Plan {
     bool few, outer;
