@@ -5,10 +5,13 @@
 //
 // (as sum_i p[t,i] = 1, any constant may be taken off all f_e: with their mean taken off, the difference of the two terms loses no
 // digits when the choices are used almost evenly).
+//
 // Both directions are one pass over the scores.  A row is shared by LPR lanes (a power of two), each with 16-byte pieces of it, so
 // that a wave reads whole lines whatever E is; the softmax's maximum and sum are butterflies over those lanes, in fp32.  Forward: a
 // lane adds up its columns over its rows in registers, lanes and waves meet in a fixed order, choices are counted with integer
 // LDS atomics; one workgroup joins the workgroups' parts in part order (in double).  Nothing depends on the order of arrival.
+// 2^19 x 128 bf16 with 8 choices a row: rows 53 us (168 MB, 3.2 TB/s: the exponentials are next), fold and join 5 each, backward 65 us
+// (268 MB, 4.1 TB/s).
 #include "nn_common.h"
 
 namespace {
