@@ -7,8 +7,9 @@
 //   umr::linear_act(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int act, float slope) -> Tensor
 //       weight [N, K]:     x [.., K],    bias [N],    residual [.., N] or [N]             -> [.., N]
 //       weight [G, N, K]:  x [.., G, K], bias [G, N], residual [.., G, N] or [G, N]       -> [.., G, N]
-//   umr::linear_act_z(..., bool keep_z) -> (y, z)     the same below autograd, z as umr_linear_forward keeps it (empty if not kept)
-//   umr::linear_act_backward(grad, x, weight, z, int act, float slope, bool need_x, need_w, need_b, need_r) -> (dx, dw, db, dr)
+//   umr::linear_act_z(...) -> (y, z)     the same below autograd, z as umr_linear_forward keeps it
+//   umr::linear_act_backward(grad, x, weight, z, int act, float slope, bool need_x, need_w, need_b, need_r) -> (dx, dw, db, dr),
+//       undefined (None) where not needed
 //   umr::balance_loss(Tensor scores, Tensor inds, Tensor? mask) -> (loss, counts)
 //   umr::balance_loss_coef(...) -> (loss, counts, coef)     below autograd
 //   umr::balance_loss_backward(grad, scores, mask, coef) -> Tensor
@@ -154,8 +155,7 @@ std::vector<int64_t> with_last(const Tensor &x, int64_t n) {
     return v;
 }
 
-std::tuple<Tensor, Tensor> linear_act_z(const Tensor &x, const Tensor &w, const optional<Tensor> &b, const optional<Tensor> &r, int64_t act,
-                                        double slope, bool keep_z) {
+Tensor linear_forward(const Tensor &x, const Tensor &w, const optional<Tensor> &b, const optional<Tensor> &r, int64_t act, double slope, Tensor *z) {
     const Sizes s = linear_sizes(x, w, b, r, act, slope);
     const char *who = "linear_act";
     on_gpu(x, x, who, "x");
@@ -168,21 +168,32 @@ std::tuple<Tensor, Tensor> linear_act_z(const Tensor &x, const Tensor &w, const 
     const Tensor bias = b ? b->contiguous() : Tensor();
     const Rows rr = r ? as_residual(*r, x, s.heads) : Rows();
     Tensor y = at::empty(with_last(x, s.N), x.options());
-    Tensor z = at::empty(keep_z ? y.sizes() : at::IntArrayRef({0}), options_of_z(x, act));
+    if (z) *z = at::empty(y.sizes(), options_of_z(x, act));
     const size_t bytes = umr_linear_forward_workspace_bytes(s.M, s.N, s.K, (int)s.G, dt);
     const Tensor ws = workspace(bytes, x);
     check_status(umr_linear_forward(xr.data(), xr.row, xr.head, wr.data(), wr.row, wr.head, b && s.N ? bias.const_data_ptr() : nullptr,
-                                    rr.data(), rr.row, rr.head, data_of(y), keep_z ? data_of(z) : nullptr, s.M, s.N, s.K, (int)s.G, dt, (int)act,
+                                    rr.data(), rr.row, rr.head, data_of(y), z ? data_of(*z) : nullptr, s.M, s.N, s.K, (int)s.G, dt, (int)act,
                                     (float)slope, data_of(ws), bytes, stream),
                  "umr_linear_forward");
+    return y;
+}
+
+Tensor linear_act(const Tensor &x, const Tensor &w, const optional<Tensor> &b, const optional<Tensor> &r, int64_t act, double slope) {
+    return linear_forward(x, w, b, r, act, slope, nullptr);
+}
+std::tuple<Tensor, Tensor> linear_act_z(const Tensor &x, const Tensor &w, const optional<Tensor> &b, const optional<Tensor> &r, int64_t act,
+                                        double slope) {
+    Tensor z, y = linear_forward(x, w, b, r, act, slope, &z);
     return {y, z};
 }
 
+Tensor linear_act_meta(const Tensor &x, const Tensor &w, const optional<Tensor> &b, const optional<Tensor> &r, int64_t act, double slope) {
+    return at::empty(with_last(x, linear_sizes(x, w, b, r, act, slope).N), x.options());
+}
 std::tuple<Tensor, Tensor> linear_act_z_meta(const Tensor &x, const Tensor &w, const optional<Tensor> &b, const optional<Tensor> &r, int64_t act,
-                                             double slope, bool keep_z) {
-    const Sizes s = linear_sizes(x, w, b, r, act, slope);
-    Tensor y = at::empty(with_last(x, s.N), x.options());
-    return {y, at::empty(keep_z ? y.sizes() : at::IntArrayRef({0}), options_of_z(x, act))};
+                                             double slope) {
+    Tensor y = linear_act_meta(x, w, b, r, act, slope);
+    return {y, at::empty(y.sizes(), options_of_z(x, act))};
 }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> linear_act_backward(const Tensor &grad, const Tensor &x, const Tensor &w, const Tensor &z, int64_t act,
@@ -202,8 +213,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> linear_act_backward(const Tensor &gra
     const auto opt = x.options();
     const Rows gr = as_rows(grad, s.heads);
     const at::IntArrayRef row2 = w.sizes().slice(0, w.dim() - 1);                 // [N] or [G, N]
-    Tensor dx = at::empty(need_x ? x.sizes() : at::IntArrayRef({0}), opt), dw = at::empty(need_w ? w.sizes() : at::IntArrayRef({0}), opt);
-    Tensor db = at::empty(need_b ? row2 : at::IntArrayRef({0}), opt), dr = at::empty(need_r ? row2 : at::IntArrayRef({0}), opt);
+    Tensor dx, dw, db, dr;
+    if (need_x) dx = at::empty(x.sizes(), opt);
+    if (need_w) dw = at::empty(w.sizes(), opt);
+    if (need_b) db = at::empty(row2, opt);
+    if (need_r) dr = at::empty(row2, opt);
     Rows dz = gr;
     const bool derive = act != UMR_ACT_NONE && (need_x || need_w || need_b);
     if (derive || need_b || need_r) {
@@ -244,31 +258,30 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> linear_act_backward(const Tensor &gra
 std::tuple<Tensor, Tensor, Tensor, Tensor> linear_act_backward_meta(const Tensor &grad, const Tensor &x, const Tensor &w, const Tensor &z, int64_t act,
                                                                     double slope, bool need_x, bool need_w, bool need_b, bool need_r) {
     const auto opt = x.options();
-    const at::IntArrayRef none({0}), row2 = w.sizes().slice(0, w.dim() - 1);
-    return {at::empty(need_x ? x.sizes() : none, opt), at::empty(need_w ? w.sizes() : none, opt), at::empty(need_b ? row2 : none, opt),
-            at::empty(need_r ? row2 : none, opt)};
+    const at::IntArrayRef row2 = w.sizes().slice(0, w.dim() - 1);
+    return {need_x ? at::empty(x.sizes(), opt) : Tensor(), need_w ? at::empty(w.sizes(), opt) : Tensor(), need_b ? at::empty(row2, opt) : Tensor(),
+            need_r ? at::empty(row2, opt) : Tensor()};
 }
 
 template <class Signature> auto typed(const char *name) {
     return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
 }
 
+enum { HAS_BIAS = 256, HAS_RESIDUAL = 512, ROW_RESIDUAL = 1024 };       // above the activation, in one saved number
+
 struct LinearAct : public torch::autograd::Function<LinearAct> {
     static Variable forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const optional<Tensor> &b, const optional<Tensor> &r, int64_t act,
-                            double slope, bool track) {
+                            double slope) {
         at::AutoDispatchBelowADInplaceOrView below;
-        static const auto op = typed<decltype(linear_act_z)>("umr::linear_act_z");
+        static const auto plain = typed<decltype(linear_act)>("umr::linear_act");
+        static const auto with_z = typed<decltype(linear_act_z)>("umr::linear_act_z");
         // act' needs the pre-activation -- or, for the two kinked ones without a residual, only its sign, which is the output's
-        const bool keep_z = track && act != UMR_ACT_NONE && !(kinked(act) && !r);
-        auto [y, z] = op.call(x, w, b, r, act, slope, keep_z);
-        if (track) {
-            ctx->save_for_backward({x, w, act == UMR_ACT_NONE ? Tensor() : keep_z ? z : y});
-            ctx->saved_data["act"] = act;
-            ctx->saved_data["slope"] = slope;
-            ctx->saved_data["row_residual"] = r && r->dim() != x.dim();
-            ctx->saved_data["bias"] = b.has_value();
-            ctx->saved_data["residual"] = r.has_value();
-        }
+        Tensor y, z;
+        if (act != UMR_ACT_NONE && !(kinked(act) && !r)) std::tie(y, z) = with_z.call(x, w, b, r, act, slope);
+        else y = plain.call(x, w, b, r, act, slope);
+        ctx->save_for_backward({x, w, act == UMR_ACT_NONE ? Tensor() : z.defined() ? z : y});
+        ctx->saved_data["act"] = act | (b ? HAS_BIAS : 0) | (r ? HAS_RESIDUAL : 0) | (r && r->dim() != x.dim() ? ROW_RESIDUAL : 0);
+        ctx->saved_data["slope"] = slope;
         return y;
     }
 
@@ -276,16 +289,15 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
         static const auto op = typed<decltype(linear_act_backward)>("umr::linear_act_backward");
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1], &g = grads[0];
-        const int64_t act = ctx->saved_data["act"].toInt();
-        const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["residual"].toBool(), row = ctx->saved_data["row_residual"].toBool();
+        const int64_t kept = ctx->saved_data["act"].toInt(), act = kept & 255;
+        const bool has_b = kept & HAS_BIAS, row = kept & ROW_RESIDUAL;
         // needs_input_grad counts the tensors that were passed, in their order
         const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = has_b && ctx->needs_input_grad(2),
-                   nr = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
-        const Tensor z = act == UMR_ACT_NONE ? g : saved[2];
+                   nr = (kept & HAS_RESIDUAL) && ctx->needs_input_grad(has_b ? 3 : 2);
         Tensor dx, dw, db, dr;
         if (nx || nw || nb || (nr && row))
-            std::tie(dx, dw, db, dr) = op.call(g, x, w, z, act, ctx->saved_data["slope"].toDouble(), nx, nw, nb, nr && row);
-        return {nx ? dx : Tensor(), nw ? dw : Tensor(), nb ? db : Tensor(), nr ? (row ? dr : g) : Tensor(), Tensor(), Tensor(), Tensor()};
+            std::tie(dx, dw, db, dr) = op.call(g, x, w, act == UMR_ACT_NONE ? g : saved[2], act, ctx->saved_data["slope"].toDouble(), nx, nw, nb, nr && row);
+        return {dx, dw, db, nr ? (row ? dr : g) : Tensor(), Tensor(), Tensor()};
     }
 };
 
@@ -293,20 +305,10 @@ bool tracked(const Tensor &a) { return a.requires_grad(); }
 bool tracked(const optional<Tensor> &a) { return a && a->requires_grad(); }
 
 Tensor linear_act_autograd(const Tensor &x, const Tensor &w, const optional<Tensor> &b, const optional<Tensor> &r, int64_t act, double slope) {
-    const bool track = at::GradMode::is_enabled() && (tracked(x) || tracked(w) || tracked(b) || tracked(r));
-    if (!track) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        static const auto op = typed<decltype(linear_act_z)>("umr::linear_act_z");
-        return std::get<0>(op.call(x, w, b, r, act, slope, false));
-    }
-    return LinearAct::apply(x, w, b, r, act, slope, track);
-}
-
-Tensor linear_act(const Tensor &x, const Tensor &w, const optional<Tensor> &b, const optional<Tensor> &r, int64_t act, double slope) {
-    return std::get<0>(linear_act_z(x, w, b, r, act, slope, false));
-}
-Tensor linear_act_meta(const Tensor &x, const Tensor &w, const optional<Tensor> &b, const optional<Tensor> &r, int64_t act, double slope) {
-    return std::get<0>(linear_act_z_meta(x, w, b, r, act, slope, false));
+    if (at::GradMode::is_enabled() && (tracked(x) || tracked(w) || tracked(b) || tracked(r))) return LinearAct::apply(x, w, b, r, act, slope);
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = typed<decltype(linear_act)>("umr::linear_act");
+    return op.call(x, w, b, r, act, slope);
 }
 
 // ---------------------------------------------------------------------------------------------- balance_loss
@@ -426,7 +428,7 @@ Tensor balance_loss_backward_once(const Tensor &grad, const Tensor &z, const opt
 
 TORCH_LIBRARY_FRAGMENT(umr, m) {
     m.def("linear_act(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int act, float slope) -> Tensor");
-    m.def("linear_act_z(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int act, float slope, bool keep_z) -> (Tensor, Tensor)");
+    m.def("linear_act_z(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int act, float slope) -> (Tensor, Tensor)");
     m.def("linear_act_backward(Tensor grad, Tensor x, Tensor weight, Tensor z, int act, float slope, bool need_x, bool need_w, bool need_b, "
           "bool need_r) -> (Tensor, Tensor, Tensor, Tensor)");
     m.def("balance_loss(Tensor scores, Tensor inds, Tensor? mask) -> (Tensor, Tensor)");
