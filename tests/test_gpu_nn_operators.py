@@ -36,6 +36,22 @@ def test_linear_largest_tiles_against_64_bits(dtype):
     C.check_linear(_lib(), 77, 1, 4100, 4099, dtype, "none", device=DEV, parts=("weight",))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_linear_largest_tiles_long_contraction_against_64_bits(dtype):
+    """as above, over contractions of at least 512, with a cut last step"""
+    C.check_linear(_lib(), 4100, 1, 4099, 523, dtype, "gelu", device=DEV, pad=1, parts=("forward",))
+    C.check_linear(_lib(), 4100, 1, 517, 4099, dtype, "none", device=DEV, parts=("input",))
+    C.check_linear(_lib(), 541, 1, 4100, 4099, dtype, "none", device=DEV, parts=("weight",))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M,G,N,K", [(1, 1, 64, 64), (16, 2, 65, 131), (17, 1, 4100, 2049), (31, 1, 2899, 2901), (32, 3, 1500, 2000), (33, 1, 2049, 4099),
+                                     (64, 1, 2899, 2901)])
+def test_linear_weight_gradient_of_few_rows_against_64_bits(M, G, N, K, dtype):
+    """outer products: up to 16 rows of any result, up to 64 of a large one, and what goes to the tiles next to them"""
+    C.check_linear(_lib(), M, G, N, K, dtype, "none", device=DEV, parts=("weight",))
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("act", list(H.ACT))
 def test_linear_activations(act, dtype):

@@ -9,8 +9,15 @@ namespace {
 Plan plan(int kind, long nq, long np, long nc, int G, int dtype) {
     Plan pl;
     const int es = dtype == UMR_F32 ? 4 : 2;
+    // Few rows, streamed weights against tiles: fp32 8192 x 8192 of 32 rows 67 / 139 us forward, 74 / 130 dx, of 64 rows 125 / 143, 107 /
+    // 132; bf16 of 64 rows 57 / 75, 45 / 80; at 1024 x 1024 the two are within 5 us of each other.
     pl.few = kind != GRAD_WEIGHT && nq <= 64;
-    pl.outer = kind == GRAD_WEIGHT && nc <= 64 && np >= 64 && nq >= 64 && ceil_div(nq, 64) <= 65535;
+    // A short contraction, outer products against the best tile: up to 16 rows 1024 x 1024 4.7 / 5.5 us, 8192 x 8192 45 / 100, bf16 29 /
+    // 73.  Beyond, the longer column gathers have to be paid for by a large result: fp32 of 32 rows 1024 x 1024 6.8 / 5.2, 2048 x 2048
+    // 9.6 / 9.8, 4096 x 4096 19 / 26, of 64 rows 9.7 / 6.1, 13.2 / 12.5, 30 / 34, 8192 x 8192 114 / 127; bf16 4096 x 4096 of 32 rows 20.8 /
+    // 21.4, of 64 34 / 21.
+    pl.outer = kind == GRAD_WEIGHT && np >= 64 && nq >= 64 && ceil_div(nq, 64) <= 65535 &&
+               (nc <= 16 || (nc <= (dtype == UMR_F32 ? 64 : 32) && (double)nq * np * G >= 8388608.));
     pl.tile = 0;
     long groups, step;
     if (pl.few) {
@@ -19,10 +26,13 @@ Plan plan(int kind, long nq, long np, long nc, int G, int dtype) {
     } else {
         // Rounds of the 256 CUs times the work of a tile, where a smaller tile reads more for each product.  Measured, 64 / 128 / 256
         // wide: fp32 10000 x 1011 x 350 78 / 110 us, 4096^3 1240 / 1170 us; bf16 8192 x 4096 x 4096 - / 370 / 300 us, 32 heads of
-        // 333 x 512 x 1024 40 / 35 / 45 us; fp16 777 x 1001 x 515 12 / 19 us
+        // 333 x 512 x 1024 40 / 35 / 45 us; fp16 777 x 1001 x 515 12 / 19 us.  The widest tile starts and ends most slowly, so it has
+        // to find a contraction of 512: 8192 x 8192 of 128 fp32 199 / 219 us, 256 343 / 353, 512 651 / 630; bf16 of 64 - / 71 / 104,
+        // 256 - / 111 / 133, 512 - / 176 / 173.
+        const int widest = (dtype == UMR_F32 ? T128x128 : T256x256) - (nc < 512);
         double best = 0;
         groups = 1;
-        for (int i = T64x64; i <= (dtype == UMR_F32 ? T128x128 : T256x256); ++i) {
+        for (int i = T64x64; i <= widest; ++i) {
             const long w = TILE[i], n = ceil_div(nq, w) * ceil_div(np, w) * G;
             const double cost = (double)ceil_div(n, 256) * (w * w + (dtype == UMR_F32 ? 16 : 128) * w);
             if (i == T64x64 || cost < best) { best = cost; pl.tile = i; groups = n; }

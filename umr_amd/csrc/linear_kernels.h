@@ -466,16 +466,16 @@ __global__ __launch_bounds__(64 * NQ * NP, 2) void k_linear_tile(Product pr, Epi
 // ------------------------------------------------------------------------------------------------ few rows: weights straight to the matrix unit
 // q <= 16 QT.  A workgroup owns 32 (fast) or 64 (slow) columns p; its 8 waves share out the contraction, add up in LDS and finish.
 // The weights are the traffic: each byte is loaded once, 16 bytes a lane, and goes to the matrix unit from registers; the rows of
-// Q come from L2 again for every workgroup.  fp32 8192 x 8192: 51 us at one row (5.3 TB/s of weights), 58 at 16, 70 at 32, 113 at 64;
-// bf16 34 us at 16 rows.  The slow form (dx): 43 us at 16 rows, part of the weights still in the memory-side cache.
-template <class T, int QT, int NW> __global__ __launch_bounds__(64 * NW) void k_linear_few(Product pr, Epilogue e) {
+// Q come from L2 again for every workgroup.  fp32 8192 x 8192: 48 us at one row (5.6 TB/s of weights), 50 at 16, 67 at 32, 125 at 64
+// (16 waves: 50, 54, 71, 113; at 4096 x 4096 18, 19, 24, 37 against 17, 19, 22, 35 with 8); bf16 34 us at 16 rows.  The slow form (dx): 43 us at 16 rows, part of the weights still in the memory-side cache.
+template <class T, int QT> __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(Product pr, Epilogue e) {
     constexpr int V = 16 / (int)sizeof(T), PT = 2, STEP = 4 * V, U = QT > 2 ? 1 : 2;     // STEP: contraction of one wave load (64 bytes a row)
-    __shared__ __attribute__((aligned(16))) float red[NW][16 * QT][36];
+    __shared__ __attribute__((aligned(16))) float red[FEW_WAVES][16 * QT][36];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l16 = lane & 15, h = lane >> 4;
     const int split = blockIdx.y, g = blockIdx.z;
     const long p0 = (long)blockIdx.x * 32;
     const long sb = split * pr.c_split, se = sb + pr.c_split < pr.nc ? sb + pr.c_split : pr.nc;
-    long per = (se - sb + NW - 1) / NW;
+    long per = (se - sb + FEW_WAVES - 1) / FEW_WAVES;
     per = (per + STEP - 1) / STEP * STEP;
     const long cb = sb + wave * per, ce = cb + per < se ? cb + per : se;
     const T *P = (const T *)pr.P.data + g * pr.P.head, *Q = (const T *)pr.Q.data + g * pr.Q.head;
@@ -520,8 +520,9 @@ template <class T, int QT, int NW> __global__ __launch_bounds__(64 * NW) void k_
     if (blocks > 0) {
         Block even, odd;
         // workgroups start at different places and wrap around: started together, all would ask L2 for the
-        // same few lines of Q at once (one row of 8192: 69 -> 51 us; with more rows of Q the lines are many anyway)
-        const long start = QT == 1 ? blockIdx.x % blocks : 0;
+        // same few lines of Q at once (fp32 8192 x 8192: one row 69 -> 51 us, 32 rows 97 -> 67; with 64 rows the lines are many
+        // anyway, and what neighbours share in the cache counts for more: 8192 x 12000 164 us against 174 with the stagger)
+        const long start = QT <= 2 ? blockIdx.x % blocks : 0;
         auto place = [&](long i) { return cb + (i + start < blocks ? i + start : i + start - blocks) * (U * STEP); };
         load(even, place(0));
         long i = 0;
@@ -554,11 +555,11 @@ template <class T, int QT, int NW> __global__ __launch_bounds__(64 * NW) void k_
 #pragma unroll
         for (int b = 0; b < QT; ++b) *(f32x4 *)&red[wave][b * 16 + l16][a * 16 + 4 * h] = acc[a][b];
     __syncthreads();
-    for (int i = t; i < 16 * QT * 8; i += 64 * NW) {
+    for (int i = t; i < 16 * QT * 8; i += 64 * FEW_WAVES) {
         const int q = i >> 3, p = (i & 7) * 4;
         f32x4 s = *(const f32x4 *)&red[0][q][p];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) {
+        for (int w = 1; w < FEW_WAVES; ++w) {
             const f32x4 o = *(const f32x4 *)&red[w][q][p];
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[j] += o[j];
@@ -656,7 +657,7 @@ template <class T, int QT> __global__ __launch_bounds__(64 * FEW_WAVES) void k_l
 // operands are slow, so that a lane gathers the contraction values of one column (they come from L2).  Here the operand whose
 // columns run along memory is the matrix instruction's second: 32 lanes then hold 32 neighbours (of 16 bits: 32 pairs of them) and a
 // store of 4 bytes a lane writes two whole lines of 128 bytes.  8192 x 8192 fp32 of 16 rows: 54 us, streamed 46 (5.9 TB/s; results of
-// 64 MB and more are streamed: they do not fit the caches, and what was there stays); 64 x 64 tiles through LDS 94.
+// 64 MB and more are streamed: they do not fit the caches, and what was there stays); 64 x 64 tiles through LDS 100.
 template <class T, bool STREAM> __global__ __launch_bounds__(256) void k_linear_outer(Product pr, T *out, long o_row, long o_head) {
     constexpr bool WORDS = sizeof(T) == 4;
     constexpr int V = 16 / (int)sizeof(T), STEP = 2 * V;
@@ -821,9 +822,7 @@ template <class T, int NQ, int NP, int FQ, int FP> int launch_tile(int kind, con
 
 template <class T, int QT> int launch_few(int kind, const Product &pr, const Epilogue &e, hipStream_t st) {
     const dim3 grid((unsigned)ceil_div(pr.np, kind == FORWARD ? 32 : 64), pr.S, pr.G);
-    const bool deep = pr.c_split >= 16 * 8 * (64 / (long)sizeof(T));      // 16 waves with at least 8 loads of a row each
-    if (kind == FORWARD && deep) UMR_LAUNCH((k_linear_few<T, QT, 16>), grid, 64 * 16, 0, st, pr, e);
-    else if (kind == FORWARD) UMR_LAUNCH((k_linear_few<T, QT, 8>), grid, 64 * 8, 0, st, pr, e);
+    if (kind == FORWARD) UMR_LAUNCH((k_linear_few<T, QT>), grid, 64 * FEW_WAVES, 0, st, pr, e);
     else UMR_LAUNCH((k_linear_few_slow<T, QT>), grid, 64 * FEW_WAVES, 0, st, pr, e);
     return umr_launch_status();
 }
