@@ -1,0 +1,36 @@
+"""CPU tests of umr_amd.model's rewriting of layers (fuse_linears, fold_for_inference): networks that hold more than plain nn.Linear
+layers compute what they computed before.  Host tensors run plain torch, so values are compared bit for bit where the operations are
+the same ones."""
+import copy
+
+import pytest
+import torch
+from torch import nn
+
+from umr_amd import model as M
+
+
+def _same(net, rewritten, x, exact=True):
+    a, b = net(x), rewritten(x)
+    if exact:
+        assert torch.equal(a, b)
+    else:       # folded in 64 bits: the same numbers in another order of operations
+        assert float((a - b).abs().max()) <= 1e-12 * max(1.0, float(a.abs().max()))
+
+
+class _Doubled(nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+@pytest.mark.parametrize("kind", ["subclass", "weight_norm", "spectral_norm"])
+def test_fused_net_keeps_the_activation_behind_a_layer_of_another_class(kind):
+    """a subclass of nn.Linear, a layer with a parametrization (torch gives it a class of its own): left alone, with its LeakyReLU"""
+    torch.manual_seed(0)
+    make = {"subclass": lambda: _Doubled(5, 6), "weight_norm": lambda: nn.utils.parametrizations.weight_norm(nn.Linear(5, 6)),
+            "spectral_norm": lambda: nn.utils.parametrizations.spectral_norm(nn.Linear(5, 6))}[kind]
+    net = nn.Sequential(make(), nn.LeakyReLU(0.2), nn.Linear(6, 4), nn.LeakyReLU(0.1)).eval()
+    fused = M.fuse_linears(copy.deepcopy(net))
+    assert type(fused[0]) is type(net[0]) and type(fused[1]) is nn.LeakyReLU
+    assert type(fused[2]) is M.Linear and fused[2].activation == "leaky_relu" and type(fused[3]) is nn.Identity
+    _same(net, fused, torch.randn(7, 5))

@@ -91,14 +91,16 @@ class Linear(nn.Linear):
 
 def fuse_linears(net):
     """Turn every nn.Linear of `net` into Linear, in place, and let it apply a LeakyReLU that directly follows it in a Sequential
-    (nn.Identity takes that place: module names, parameters and state_dict keys stay).  Returns net."""
+    (nn.Identity takes that place: module names, parameters and state_dict keys stay).  Returns net.
+
+    Left as it is, with what follows it: a layer of any other class (a subclass of nn.Linear, a layer with a parametrization)."""
     for m in list(net.modules()):
         kids = list(m._modules.items())
         for k, (_, a) in enumerate(kids):
-            if not isinstance(a, nn.Linear) or getattr(a, "activation", "none") != "none":
-                continue
             if type(a) is nn.Linear:
                 a.__class__ = Linear
+            if type(a) is not Linear or a.activation != "none":
+                continue
             if isinstance(m, nn.Sequential) and k + 1 < len(kids) and type(kids[k + 1][1]) is nn.LeakyReLU:
                 a.activation, a.slope = "leaky_relu", float(kids[k + 1][1].negative_slope)
                 m._modules[kids[k + 1][0]] = nn.Identity()
