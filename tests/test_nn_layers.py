@@ -34,3 +34,19 @@ def test_fused_net_keeps_the_activation_behind_a_layer_of_another_class(kind):
     assert type(fused[0]) is type(net[0]) and type(fused[1]) is nn.LeakyReLU
     assert type(fused[2]) is M.Linear and fused[2].activation == "leaky_relu" and type(fused[3]) is nn.Identity
     _same(net, fused, torch.randn(7, 5))
+
+
+def test_fused_net_applies_no_activation_to_a_layers_other_uses():
+    """one layer in several places, with a LeakyReLU behind it in some of them: each place keeps its own activation"""
+    torch.manual_seed(1)
+    layer = nn.Linear(5, 5)
+    for net in (nn.Sequential(layer, nn.LeakyReLU(0.2), layer), nn.Sequential(layer, nn.LeakyReLU(0.2), layer, nn.LeakyReLU(0.4)),
+                nn.Sequential(nn.Sequential(layer, nn.LeakyReLU(0.2)), nn.Sequential(layer, nn.LeakyReLU(0.2))),
+                nn.Sequential(nn.Sequential(layer, nn.LeakyReLU(0.2)), nn.ModuleDict(dict(other=layer))["other"])):
+        net = copy.deepcopy(net)
+        _same(net, M.fuse_linears(copy.deepcopy(net)), torch.randn(7, 5))
+    inner = nn.Sequential(nn.Linear(5, 5), nn.LeakyReLU(0.2))               # a block in several places: fused once, the same everywhere
+    net = nn.Sequential(inner, inner)
+    fused = M.fuse_linears(copy.deepcopy(net))
+    assert fused[1][0].activation == "leaky_relu"
+    _same(net, fused, torch.randn(7, 5))

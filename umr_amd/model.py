@@ -12,6 +12,7 @@ torchvision is not available here, so the ResNet-18 trunk (cub_mesh.py:53-74) is
 with random initialisation (the pretrained weights are not obtainable offline).  Parameter shapes follow the
 reference, so the gradient all-reduce volume (~85 M fp32) is the reference's.
 """
+from collections import Counter
 from types import SimpleNamespace
 
 import numpy as np
@@ -93,13 +94,15 @@ def fuse_linears(net):
     """Turn every nn.Linear of `net` into Linear, in place, and let it apply a LeakyReLU that directly follows it in a Sequential
     (nn.Identity takes that place: module names, parameters and state_dict keys stay).  Returns net.
 
-    Left as it is, with what follows it: a layer of any other class (a subclass of nn.Linear, a layer with a parametrization)."""
+    Left as it is, with what follows it: a layer of any other class (a subclass of nn.Linear, a layer with a parametrization).  A
+    layer that is registered in several places applies no activation itself: another place may have another one behind it."""
+    uses = Counter(kid for m in net.modules() for kid in m._modules.values())
     for m in list(net.modules()):
         kids = list(m._modules.items())
         for k, (_, a) in enumerate(kids):
             if type(a) is nn.Linear:
                 a.__class__ = Linear
-            if type(a) is not Linear or a.activation != "none":
+            if type(a) is not Linear or a.activation != "none" or uses[a] > 1:
                 continue
             if isinstance(m, nn.Sequential) and k + 1 < len(kids) and type(kids[k + 1][1]) is nn.LeakyReLU:
                 a.activation, a.slope = "leaky_relu", float(kids[k + 1][1].negative_slope)
