@@ -50,3 +50,14 @@ def test_fused_net_applies_no_activation_to_a_layers_other_uses():
     fused = M.fuse_linears(copy.deepcopy(net))
     assert fused[1][0].activation == "leaky_relu"
     _same(net, fused, torch.randn(7, 5))
+
+
+class _Skips(nn.Sequential):
+    def forward(self, x):                                                   # another order than a Sequential's
+        return self[1](x) + self[0](x)
+
+
+def test_fused_net_leaves_a_sequential_with_a_forward_of_its_own():
+    torch.manual_seed(2)
+    net = _Skips(nn.Linear(5, 5), nn.LeakyReLU(0.2))
+    _same(net, M.fuse_linears(copy.deepcopy(net)), torch.randn(7, 5))

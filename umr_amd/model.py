@@ -90,23 +90,28 @@ class Linear(nn.Linear):
         return _linear_act(x, self.weight, self.bias, self.activation, self.slope)
 
 
+def _chains(m):
+    """[(name, child)] of a Sequential that calls its children one after the other, [] of any other module."""
+    return list(m._modules.items()) if isinstance(m, nn.Sequential) and type(m).forward is nn.Sequential.forward else []
+
+
 def fuse_linears(net):
     """Turn every nn.Linear of `net` into Linear, in place, and let it apply a LeakyReLU that directly follows it in a Sequential
     (nn.Identity takes that place: module names, parameters and state_dict keys stay).  Returns net.
 
     Left as it is, with what follows it: a layer of any other class (a subclass of nn.Linear, a layer with a parametrization).  A
-    layer that is registered in several places applies no activation itself: another place may have another one behind it."""
+    layer that is registered in several places applies no activation itself: another place may have another one behind it.  A
+    Sequential with a forward of its own keeps its LeakyReLUs: what follows what is not known there."""
     uses = Counter(kid for m in net.modules() for kid in m._modules.values())
     for m in list(net.modules()):
-        kids = list(m._modules.items())
-        for k, (_, a) in enumerate(kids):
-            if type(a) is nn.Linear:
-                a.__class__ = Linear
-            if type(a) is not Linear or a.activation != "none" or uses[a] > 1:
-                continue
-            if isinstance(m, nn.Sequential) and k + 1 < len(kids) and type(kids[k + 1][1]) is nn.LeakyReLU:
-                a.activation, a.slope = "leaky_relu", float(kids[k + 1][1].negative_slope)
-                m._modules[kids[k + 1][0]] = nn.Identity()
+        if type(m) is nn.Linear:
+            m.__class__ = Linear
+    for m in list(net.modules()):
+        kids = _chains(m)
+        for (_, a), (name, b) in zip(kids, kids[1:]):
+            if type(a) is Linear and a.activation == "none" and uses[a] == 1 and type(b) is nn.LeakyReLU:
+                a.activation, a.slope = "leaky_relu", float(b.negative_slope)
+                m._modules[name] = nn.Identity()
     return net
 
 
