@@ -61,3 +61,21 @@ def test_fused_net_leaves_a_sequential_with_a_forward_of_its_own():
     torch.manual_seed(2)
     net = _Skips(nn.Linear(5, 5), nn.LeakyReLU(0.2))
     _same(net, M.fuse_linears(copy.deepcopy(net)), torch.randn(7, 5))
+
+
+def test_fused_net_keeps_what_hooks_see():
+    """a hook on a layer's output or its gradient sees the product, not the activation; a hook on the LeakyReLU still runs"""
+    torch.manual_seed(3)
+    for where, hook in ((0, "register_forward_hook"), (0, "register_full_backward_hook"), (1, "register_forward_hook"),
+                        (1, "register_forward_pre_hook"), (1, "register_full_backward_hook"), (1, "register_full_backward_pre_hook")):
+        seen = []
+        net = nn.Sequential(nn.Linear(5, 6), nn.LeakyReLU(0.2))
+        plain = copy.deepcopy(net)
+        for m in (plain, net):
+            getattr(m[where], hook)(lambda mod, *a: seen.append([t.detach().clone() for v in a for t in (v if isinstance(v, tuple) else (v,)) if t is not None]))
+        fused = M.fuse_linears(net)
+        x = torch.randn(7, 5)
+        for m in (plain, fused):
+            m(x.clone().requires_grad_(True)).square().sum().backward()
+        assert len(seen) == 2, hook
+        assert len(seen[0]) == len(seen[1]) and all(torch.equal(a, b) for a, b in zip(*seen)), hook

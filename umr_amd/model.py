@@ -95,13 +95,19 @@ def _chains(m):
     return list(m._modules.items()) if isinstance(m, nn.Sequential) and type(m).forward is nn.Sequential.forward else []
 
 
+def _hooked(m, inputs_too=True):
+    """A hook looks at this module's output or gradient (inputs_too: or at its input)."""
+    return bool(m._forward_hooks or m._backward_hooks or m._backward_pre_hooks or inputs_too and m._forward_pre_hooks)
+
+
 def fuse_linears(net):
     """Turn every nn.Linear of `net` into Linear, in place, and let it apply a LeakyReLU that directly follows it in a Sequential
     (nn.Identity takes that place: module names, parameters and state_dict keys stay).  Returns net.
 
     Left as it is, with what follows it: a layer of any other class (a subclass of nn.Linear, a layer with a parametrization).  A
     layer that is registered in several places applies no activation itself: another place may have another one behind it.  A
-    Sequential with a forward of its own keeps its LeakyReLUs: what follows what is not known there."""
+    Sequential with a forward of its own keeps its LeakyReLUs: what follows what is not known there.  So does a pair whose values
+    between product and activation a hook asks for; one registered later sees the activated output."""
     uses = Counter(kid for m in net.modules() for kid in m._modules.values())
     for m in list(net.modules()):
         if type(m) is nn.Linear:
@@ -109,7 +115,8 @@ def fuse_linears(net):
     for m in list(net.modules()):
         kids = _chains(m)
         for (_, a), (name, b) in zip(kids, kids[1:]):
-            if type(a) is Linear and a.activation == "none" and uses[a] == 1 and type(b) is nn.LeakyReLU:
+            if type(a) is Linear and a.activation == "none" and uses[a] == 1 and type(b) is nn.LeakyReLU and \
+                    not _hooked(a, inputs_too=False) and not _hooked(b):
                 a.activation, a.slope = "leaky_relu", float(b.negative_slope)
                 m._modules[name] = nn.Identity()
     return net
