@@ -79,3 +79,14 @@ def test_fused_net_keeps_what_hooks_see():
             m(x.clone().requires_grad_(True)).square().sum().backward()
         assert len(seen) == 2, hook
         assert len(seen[0]) == len(seen[1]) and all(torch.equal(a, b) for a, b in zip(*seen)), hook
+
+
+@pytest.mark.parametrize("slope", [-0.25, float("nan")])
+def test_fused_net_keeps_a_leaky_relu_that_the_operator_refuses(slope):
+    """linear_act takes slopes >= 0: the sign of its output has to be that of the pre-activation"""
+    torch.manual_seed(4)
+    net = nn.Sequential(nn.Linear(5, 6), nn.LeakyReLU(slope))
+    fused = M.fuse_linears(copy.deepcopy(net))
+    assert fused[0].activation == "none" and type(fused[1]) is nn.LeakyReLU
+    x = torch.randn(7, 5)
+    assert torch.equal(torch.nan_to_num(net(x)), torch.nan_to_num(fused(x)))

@@ -115,7 +115,7 @@ def fuse_linears(net):
     for m in list(net.modules()):
         kids = _chains(m)
         for (_, a), (name, b) in zip(kids, kids[1:]):
-            if type(a) is Linear and a.activation == "none" and uses[a] == 1 and type(b) is nn.LeakyReLU and \
+            if type(a) is Linear and a.activation == "none" and uses[a] == 1 and type(b) is nn.LeakyReLU and b.negative_slope >= 0 and \
                     not _hooked(a, inputs_too=False) and not _hooked(b):
                 a.activation, a.slope = "leaky_relu", float(b.negative_slope)
                 m._modules[name] = nn.Identity()
