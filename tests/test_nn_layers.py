@@ -90,3 +90,22 @@ def test_fused_net_keeps_a_leaky_relu_that_the_operator_refuses(slope):
     assert fused[0].activation == "none" and type(fused[1]) is nn.LeakyReLU
     x = torch.randn(7, 5)
     assert torch.equal(torch.nan_to_num(net(x)), torch.nan_to_num(fused(x)))
+
+
+# ---------------------------------------------------------------------------------------------- fold_for_inference
+def _normed(n, **kw):
+    bn = nn.BatchNorm1d(n, **kw).double()
+    if bn.running_mean is not None:
+        bn.running_mean.normal_(0, 0.3), bn.running_var.uniform_(0.5, 2.0)
+    if bn.weight is not None:
+        bn.weight.data.uniform_(0.5, 1.5), bn.bias.data.normal_(0, 0.1)
+    return bn
+
+
+@pytest.mark.parametrize("kind", ["subclass", "weight_norm", "spectral_norm"])
+def test_folded_net_leaves_a_layer_of_another_class(kind):
+    torch.manual_seed(5)
+    make = {"subclass": lambda: _Doubled(5, 6), "weight_norm": lambda: nn.utils.parametrizations.weight_norm(nn.Linear(5, 6)),
+            "spectral_norm": lambda: nn.utils.parametrizations.spectral_norm(nn.Linear(5, 6))}[kind]
+    net = nn.Sequential(make().double(), _normed(6), nn.LeakyReLU(0.2)).eval()
+    _same(net, M.fold_for_inference(net), torch.randn(7, 5).double(), exact=False)

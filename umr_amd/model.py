@@ -132,7 +132,9 @@ def _fold_batch_norm(lin, bn):
 def fold_for_inference(net):
     """A copy of `net` (MeshNet or a part of it) for inference: eval mode, no gradients, every Linear + BatchNorm1d [+ LeakyReLU] of
     a Sequential folded into one layer, and the cameras of a MultiCamPredictor as three layers for all of them at once (its first
-    layer is shared input: one product; the others one product a camera, in one launch).  The weights are laid out here, once."""
+    layer is shared input: one product; the others one product a camera, in one launch).  The weights are laid out here, once.
+
+    Left as it is, with its batch norm: a layer of any other class than nn.Linear or Linear."""
     import copy
     net = copy.deepcopy(net).eval()
     for p in net.parameters():
@@ -140,7 +142,7 @@ def fold_for_inference(net):
     for m in list(net.modules()):
         kids = list(m._modules.items()) if isinstance(m, nn.Sequential) else []
         for (_, a), (name, b) in zip(kids, kids[1:]):
-            if isinstance(a, nn.Linear) and getattr(a, "activation", "none") == "none" and type(b) is nn.BatchNorm1d:
+            if type(a) in (nn.Linear, Linear) and getattr(a, "activation", "none") == "none" and type(b) is nn.BatchNorm1d:
                 w, bias = _fold_batch_norm(a, b)
                 a.weight.copy_(w)
                 a.bias.copy_(bias)
