@@ -109,3 +109,20 @@ def test_folded_net_leaves_a_layer_of_another_class(kind):
             "spectral_norm": lambda: nn.utils.parametrizations.spectral_norm(nn.Linear(5, 6))}[kind]
     net = nn.Sequential(make().double(), _normed(6), nn.LeakyReLU(0.2)).eval()
     _same(net, M.fold_for_inference(net), torch.randn(7, 5).double(), exact=False)
+
+
+def test_folded_net_folds_each_place_of_a_shared_layer_by_itself():
+    """one layer, or one weight, in front of two batch norms"""
+    torch.manual_seed(6)
+    x = torch.randn(7, 5).double()
+    layer = nn.Linear(5, 5).double()
+    net = nn.Sequential(layer, _normed(5), nn.LeakyReLU(0.2), layer, _normed(5)).eval()
+    _same(net, M.fold_for_inference(net), x, exact=False)
+    tied = nn.Linear(5, 5).double()
+    tied.weight, tied.bias = layer.weight, layer.bias
+    for other in (tied, nn.Sequential(tied, nn.LeakyReLU(0.1))):             # ... or alone
+        net = nn.Sequential(layer, _normed(5), nn.LeakyReLU(0.2), other, layer).eval()
+        _same(net, M.fold_for_inference(net), x, exact=False)
+    inner = nn.Sequential(layer, _normed(5))                                # a block in two places
+    net = nn.Sequential(inner, nn.LeakyReLU(0.2), inner).eval()
+    _same(net, M.fold_for_inference(net), x, exact=False)

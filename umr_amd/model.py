@@ -123,9 +123,13 @@ def fuse_linears(net):
 
 
 def _fold_batch_norm(lin, bn):
-    """(weight, bias) of the layer that equals bn(lin(x)) with bn's running statistics; formed in 64 bits."""
+    """The layer that equals bn(lin(x)) with bn's running statistics; formed in 64 bits.  A new one: lin, or its parameters, may serve
+    other places too."""
     s = bn.weight.double() / torch.sqrt(bn.running_var.double() + bn.eps)
-    return (lin.weight.double() * s[:, None]).to(lin.weight.dtype), ((lin.bias.double() - bn.running_mean.double()) * s + bn.bias.double()).to(lin.bias.dtype)
+    out = Linear(lin.in_features, lin.out_features, device=lin.weight.device, dtype=lin.weight.dtype)
+    out.weight.copy_(lin.weight.double() * s[:, None])
+    out.bias.copy_((lin.bias.double() - bn.running_mean.double()) * s + bn.bias.double())
+    return out.eval().requires_grad_(False)
 
 
 @torch.no_grad()
@@ -141,11 +145,9 @@ def fold_for_inference(net):
         p.requires_grad_(False)
     for m in list(net.modules()):
         kids = list(m._modules.items()) if isinstance(m, nn.Sequential) else []
-        for (_, a), (name, b) in zip(kids, kids[1:]):
+        for (layer, a), (name, b) in zip(kids, kids[1:]):
             if type(a) in (nn.Linear, Linear) and getattr(a, "activation", "none") == "none" and type(b) is nn.BatchNorm1d:
-                w, bias = _fold_batch_norm(a, b)
-                a.weight.copy_(w)
-                a.bias.copy_(bias)
+                m._modules[layer] = _fold_batch_norm(a, b)
                 del m._modules[name]                      # (the LeakyReLU now follows the Linear)
     for m in list(net.modules()):
         if isinstance(m, MultiCamPredictor):
