@@ -126,3 +126,18 @@ def test_folded_net_folds_each_place_of_a_shared_layer_by_itself():
     inner = nn.Sequential(layer, _normed(5))                                # a block in two places
     net = nn.Sequential(inner, nn.LeakyReLU(0.2), inner).eval()
     _same(net, M.fold_for_inference(net), x, exact=False)
+
+
+def test_folded_net_keeps_a_batch_norm_that_has_no_fixed_map():
+    """no bias, no affine map: folded all the same; statistics of the batch, of other dimensions than the layer's outputs: kept"""
+    torch.manual_seed(7)
+    x = torch.randn(7, 5).double()
+    for bias, kw in ((False, {}), (True, dict(affine=False)), (False, dict(affine=False))):
+        net = nn.Sequential(nn.Linear(5, 6, bias=bias).double(), _normed(6, **kw), nn.LeakyReLU(0.2)).eval()
+        folded = M.fold_for_inference(net)
+        assert len(folded) == 2
+        _same(net, folded, x, exact=False)
+    net = nn.Sequential(nn.Linear(5, 6).double(), _normed(6, track_running_stats=False)).eval()
+    _same(net, M.fold_for_inference(net), x)
+    net = nn.Sequential(nn.Linear(5, 6).double(), _normed(3)).eval()         # [B, 3, 5]: a batch norm over the middle dimension
+    _same(net, M.fold_for_inference(net), torch.randn(7, 3, 5).double())

@@ -125,10 +125,13 @@ def fuse_linears(net):
 def _fold_batch_norm(lin, bn):
     """The layer that equals bn(lin(x)) with bn's running statistics; formed in 64 bits.  A new one: lin, or its parameters, may serve
     other places too."""
-    s = bn.weight.double() / torch.sqrt(bn.running_var.double() + bn.eps)
-    out = Linear(lin.in_features, lin.out_features, device=lin.weight.device, dtype=lin.weight.dtype)
+    s = 1 / torch.sqrt(bn.running_var.double() + bn.eps)
+    if bn.weight is not None:
+        s = s * bn.weight.double()
+    shift = (0 if lin.bias is None else lin.bias.double()) - bn.running_mean.double()
+    out = nn.utils.skip_init(Linear, lin.in_features, lin.out_features, device=lin.weight.device, dtype=lin.weight.dtype)
     out.weight.copy_(lin.weight.double() * s[:, None])
-    out.bias.copy_((lin.bias.double() - bn.running_mean.double()) * s + bn.bias.double())
+    out.bias.copy_(shift * s if bn.bias is None else shift * s + bn.bias.double())
     return out.eval().requires_grad_(False)
 
 
@@ -138,7 +141,8 @@ def fold_for_inference(net):
     a Sequential folded into one layer, and the cameras of a MultiCamPredictor as three layers for all of them at once (its first
     layer is shared input: one product; the others one product a camera, in one launch).  The weights are laid out here, once.
 
-    Left as it is, with its batch norm: a layer of any other class than nn.Linear or Linear."""
+    Left as it is, with its batch norm: a layer of any other class than nn.Linear or Linear, a batch norm without running
+    statistics or over another dimension than the layer's outputs (inputs are [B, features])."""
     import copy
     net = copy.deepcopy(net).eval()
     for p in net.parameters():
@@ -146,7 +150,8 @@ def fold_for_inference(net):
     for m in list(net.modules()):
         kids = list(m._modules.items()) if isinstance(m, nn.Sequential) else []
         for (layer, a), (name, b) in zip(kids, kids[1:]):
-            if type(a) in (nn.Linear, Linear) and getattr(a, "activation", "none") == "none" and type(b) is nn.BatchNorm1d:
+            if type(a) in (nn.Linear, Linear) and getattr(a, "activation", "none") == "none" and type(b) is nn.BatchNorm1d and \
+                    b.running_mean is not None and b.num_features == a.out_features:
                 m._modules[layer] = _fold_batch_norm(a, b)
                 del m._modules[name]                      # (the LeakyReLU now follows the Linear)
     for m in list(net.modules()):
