@@ -141,3 +141,14 @@ def test_folded_net_keeps_a_batch_norm_that_has_no_fixed_map():
     _same(net, M.fold_for_inference(net), x)
     net = nn.Sequential(nn.Linear(5, 6).double(), _normed(3)).eval()         # [B, 3, 5]: a batch norm over the middle dimension
     _same(net, M.fold_for_inference(net), torch.randn(7, 3, 5).double())
+
+
+def test_folded_net_leaves_hooked_layers_and_sequentials_with_a_forward_of_their_own():
+    torch.manual_seed(8)
+    x = torch.randn(7, 5).double()
+    for where in (0, 1):
+        net = nn.Sequential(nn.Linear(5, 6).double(), _normed(6), nn.LeakyReLU(0.2)).eval()
+        net[where].register_forward_hook(lambda mod, inp, out: out + 1)
+        _same(net, M.fold_for_inference(net), x)
+    net = _Skips(nn.Linear(5, 5), _normed(5)).double().eval()
+    _same(net, M.fold_for_inference(net), x)

@@ -142,16 +142,17 @@ def fold_for_inference(net):
     layer is shared input: one product; the others one product a camera, in one launch).  The weights are laid out here, once.
 
     Left as it is, with its batch norm: a layer of any other class than nn.Linear or Linear, a batch norm without running
-    statistics or over another dimension than the layer's outputs (inputs are [B, features])."""
+    statistics or over another dimension than the layer's outputs (inputs are [B, features]), what a hook looks at, a Sequential
+    with a forward of its own."""
     import copy
     net = copy.deepcopy(net).eval()
     for p in net.parameters():
         p.requires_grad_(False)
     for m in list(net.modules()):
-        kids = list(m._modules.items()) if isinstance(m, nn.Sequential) else []
+        kids = _chains(m)
         for (layer, a), (name, b) in zip(kids, kids[1:]):
             if type(a) in (nn.Linear, Linear) and getattr(a, "activation", "none") == "none" and type(b) is nn.BatchNorm1d and \
-                    b.running_mean is not None and b.num_features == a.out_features:
+                    b.running_mean is not None and b.num_features == a.out_features and not _hooked(a) and not _hooked(b):
                 m._modules[layer] = _fold_batch_norm(a, b)
                 del m._modules[name]                      # (the LeakyReLU now follows the Linear)
     for m in list(net.modules()):
