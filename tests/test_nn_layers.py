@@ -152,3 +152,57 @@ def test_folded_net_leaves_hooked_layers_and_sequentials_with_a_forward_of_their
         _same(net, M.fold_for_inference(net), x)
     net = _Skips(nn.Linear(5, 5), _normed(5)).double().eval()
     _same(net, M.fold_for_inference(net), x)
+
+
+# ---------------------------------------------------------------------------------------------- the cameras' three layers
+def _predictor(seed=9):
+    torch.manual_seed(seed)
+    net = M.MultiCamPredictor(12, 4)
+    for m in net.modules():
+        if isinstance(m, nn.Linear):
+            m.weight.data.normal_(0, 0.3)
+        if isinstance(m, nn.BatchNorm1d):
+            m.running_mean.normal_(0, 0.3), m.running_var.uniform_(0.5, 2.0)
+    return net.double().eval()
+
+
+def _same_cameras(net, folded, feat):
+    outs = []
+    for m in (net, folded):
+        torch.manual_seed(5)
+        outs.append(m(feat, with_logits=True))
+    for a, b in zip(*outs):
+        assert a.dtype == b.dtype and float((a - b).abs().max()) <= 1e-7 * max(1.0, float(a.abs().max()))
+
+
+def test_cameras_that_differ_from_each_other_stay_apart():
+    """another slope, another scale, a layer of another class, a hook, another stack, something that is not a Camera: what three layers for
+    all cheaply cannot hold; and a predictor that is folded already"""
+    feat = torch.randn(6, 12).double()
+
+    def slope(net):
+        net.camera_predictor[2].fc_layer[0][2] = nn.LeakyReLU(0.5)
+
+    def subclass(net):
+        old, new = net.camera_predictor[1].prob_predictor, _Doubled(12, 1).double()
+        new.load_state_dict(old.state_dict())
+        net.camera_predictor[1].prob_predictor = new
+
+    def hook(net):
+        net.camera_predictor[3].trans_predictor.pred_layer.register_forward_hook(lambda m, i, o: o + 1)
+
+    def no_batch_norm(net):
+        net.camera_predictor[0].fc_layer = M.fc_stack(12, 12, 3).double().eval()
+
+    def another_norm(net):
+        net.camera_predictor[0].fc_layer[1][1] = _normed(12, track_running_stats=False)
+
+    def wrapped(net):
+        net.camera_predictor[0] = nn.Sequential(net.camera_predictor[0])
+    for change in (lambda net: None, slope, subclass, hook, no_batch_norm, another_norm, wrapped):
+        net = _predictor()
+        change(net)
+        _same_cameras(net, M.fold_for_inference(net), feat)
+    folded = M.fold_for_inference(_predictor())
+    assert isinstance(folded.camera_predictor, M.FoldedCameras)
+    _same_cameras(folded, M.fold_for_inference(folded), feat)

@@ -143,7 +143,7 @@ def fold_for_inference(net):
 
     Left as it is, with its batch norm: a layer of any other class than nn.Linear or Linear, a batch norm without running
     statistics or over another dimension than the layer's outputs (inputs are [B, features]), what a hook looks at, a Sequential
-    with a forward of its own."""
+    with a forward of its own; cameras that are not alike in everything but their parameters and scales."""
     import copy
     net = copy.deepcopy(net).eval()
     for p in net.parameters():
@@ -156,7 +156,7 @@ def fold_for_inference(net):
                 m._modules[layer] = _fold_batch_norm(a, b)
                 del m._modules[name]                      # (the LeakyReLU now follows the Linear)
     for m in list(net.modules()):
-        if isinstance(m, MultiCamPredictor):
+        if isinstance(m, MultiCamPredictor) and FoldedCameras.fits(m.camera_predictor):
             m.camera_predictor = FoldedCameras(m.camera_predictor)
     return fuse_linears(net)
 
@@ -388,11 +388,33 @@ class FoldedCameras(nn.Module):
     """The K Camera heads of a MultiCamPredictor as three layers (fold_for_inference): [B, nz] -> [B, K, 8], what
     torch.stack([camera(f) for camera in cameras], 1) gives."""
 
+    @staticmethod
+    def _last(c):
+        return [c.quat_predictor.pred_layer, c.prob_predictor, c.scale_predictor.pred_layer, c.trans_predictor.pred_layer]
+
+    @classmethod
+    def fits(cls, cameras):
+        """cameras: a ModuleList of Cameras with folded batch norms, i.e. two plain layers with one LeakyReLU each, then four"""
+        if not isinstance(cameras, nn.ModuleList) or not len(cameras):
+            return False
+        forms = set()
+        for c in cameras:
+            stack = [_chains(l) for l in c.fc_layer] if type(c) is Camera and _chains(c.fc_layer) else []
+            if len(stack) != 2 or any(len(s) != 2 or type(s[1][1]) is not nn.LeakyReLU for s in stack) or any(_hooked(m) for m in c.modules()):
+                return False
+            preds = (c.quat_predictor, c.scale_predictor, c.trans_predictor)
+            layers = [s[0][1] for s in stack] + cls._last(c)
+            if any(type(p) is not _Pred for p in preds) or any(
+                    type(l) not in (nn.Linear, Linear) or getattr(l, "activation", "none") != "none" or l.bias is None for l in layers):
+                return False
+            forms.add(tuple(s[1][1].negative_slope for s in stack) + tuple(l.weight.shape for l in layers))
+        return len(forms) == 1 and all(s >= 0 for s in next(iter(forms))[:2])
+
     def __init__(self, cameras):
         super().__init__()
         cameras = list(cameras)
         first, second = [c.fc_layer[0][0] for c in cameras], [c.fc_layer[1][0] for c in cameras]
-        last = [[c.quat_predictor.pred_layer, c.prob_predictor, c.scale_predictor.pred_layer, c.trans_predictor.pred_layer] for c in cameras]
+        last = [self._last(c) for c in cameras]
         self.register_buffer("w1", torch.cat([l.weight for l in first]))
         self.register_buffer("b1", torch.cat([l.bias for l in first]))
         self.register_buffer("w2", torch.stack([l.weight for l in second]))
