@@ -206,3 +206,24 @@ def test_cameras_that_differ_from_each_other_stay_apart():
     folded = M.fold_for_inference(_predictor())
     assert isinstance(folded.camera_predictor, M.FoldedCameras)
     _same_cameras(folded, M.fold_for_inference(folded), feat)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float64], ids=str)
+def test_folded_cameras_keep_the_networks_type_and_scales(dtype):
+    """outputs in the type of the network, before and after a conversion; scale_lr and scale_bias are constants of that type's arithmetic, as
+    in Camera; cameras with scales of their own stay apart"""
+    net = _predictor()
+    for k, c in enumerate(net.camera_predictor):
+        c.scale_lr, c.scale_bias = 0.05 + 0.01 * k, 1.0 / 3
+    _same_cameras(net, M.fold_for_inference(net), torch.randn(6, 12).double())
+    for c in net.camera_predictor:
+        c.scale_lr = 0.05
+    feat = torch.randn(6, 12).to(dtype)
+    before, after = M.fold_for_inference(copy.deepcopy(net).to(dtype)), M.fold_for_inference(net).to(dtype)
+    for folded in (before, after):
+        outs = [m(feat, with_logits=True) for m in (copy.deepcopy(net).to(dtype), folded)]
+        for i in (3, 4, 5):
+            a, b = outs[0][i], outs[1][i]
+            assert a.dtype == b.dtype == dtype
+            if dtype is torch.float64:                                       # (sums in another order)
+                assert float((a - b).abs().max()) <= 1e-13 * max(1.0, float(a.abs().max()))

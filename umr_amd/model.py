@@ -143,7 +143,7 @@ def fold_for_inference(net):
 
     Left as it is, with its batch norm: a layer of any other class than nn.Linear or Linear, a batch norm without running
     statistics or over another dimension than the layer's outputs (inputs are [B, features]), what a hook looks at, a Sequential
-    with a forward of its own; cameras that are not alike in everything but their parameters and scales."""
+    with a forward of its own; cameras that are not alike in everything but their parameters."""
     import copy
     net = copy.deepcopy(net).eval()
     for p in net.parameters():
@@ -407,7 +407,7 @@ class FoldedCameras(nn.Module):
             if any(type(p) is not _Pred for p in preds) or any(
                     type(l) not in (nn.Linear, Linear) or getattr(l, "activation", "none") != "none" or l.bias is None for l in layers):
                 return False
-            forms.add(tuple(s[1][1].negative_slope for s in stack) + tuple(l.weight.shape for l in layers))
+            forms.add(tuple(s[1][1].negative_slope for s in stack) + (c.scale_lr, c.scale_bias) + tuple(l.weight.shape for l in layers))
         return len(forms) == 1 and all(s >= 0 for s in next(iter(forms))[:2])
 
     def __init__(self, cameras):
@@ -421,8 +421,7 @@ class FoldedCameras(nn.Module):
         self.register_buffer("b2", torch.stack([l.bias for l in second]))
         self.register_buffer("w3", torch.stack([torch.cat([l.weight for l in ls]) for ls in last]))
         self.register_buffer("b3", torch.stack([torch.cat([l.bias for l in ls]) for ls in last]))
-        self.register_buffer("scale_lr", torch.tensor([float(c.scale_lr) for c in cameras], device=self.w1.device)[:, None])
-        self.register_buffer("scale_bias", torch.tensor([float(c.scale_bias) for c in cameras], device=self.w1.device)[:, None])
+        self.scale_lr, self.scale_bias = cameras[0].scale_lr, cameras[0].scale_bias
         self.slope = [float(c.fc_layer[i][1].negative_slope) for c in cameras[:1] for i in (0, 1)]
 
     def forward(self, f):
