@@ -301,10 +301,19 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     }
 };
 
+// A tangent (torch.autograd.forward_ad, torch.func.jvp) needs no requires_grad and passes no_grad: refused wherever one arrives,
+// or the result would come without it.
+void no_tangent(const char *name, std::initializer_list<const Tensor *> inputs) {
+    for (const Tensor *t : inputs)
+        TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), "umr_amd: ", name, " has no forward-mode derivative");
+}
+const Tensor *given(const optional<Tensor> &t) { return t ? &*t : nullptr; }
+
 bool tracked(const Tensor &a) { return a.requires_grad(); }
 bool tracked(const optional<Tensor> &a) { return a && a->requires_grad(); }
 
 Tensor linear_act_autograd(const Tensor &x, const Tensor &w, const optional<Tensor> &b, const optional<Tensor> &r, int64_t act, double slope) {
+    no_tangent("linear_act", {&x, &w, given(b), given(r)});
     if (at::GradMode::is_enabled() && (tracked(x) || tracked(w) || tracked(b) || tracked(r))) return LinearAct::apply(x, w, b, r, act, slope);
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = typed<decltype(linear_act)>("umr::linear_act");
@@ -388,6 +397,7 @@ struct BalanceLoss : public torch::autograd::Function<BalanceLoss> {
 };
 
 std::tuple<Tensor, Tensor> balance_loss_autograd(const Tensor &z, const Tensor &inds, const optional<Tensor> &mask) {
+    no_tangent("balance_loss", {&z});
     if (at::GradMode::is_enabled() && z.requires_grad()) {
         auto out = BalanceLoss::apply(z, inds, mask);
         return {out[0], out[1]};
@@ -412,12 +422,14 @@ void once_only(bool any, const char *name) {
 }
 std::tuple<Tensor, Tensor, Tensor, Tensor> linear_act_backward_once(const Tensor &grad, const Tensor &x, const Tensor &w, const Tensor &z, int64_t act,
                                                                     double slope, bool nx, bool nw, bool nb, bool nr) {
+    no_tangent("the gradient of linear_act", {&grad, &x, &w, &z});
     once_only(tracked(grad) || tracked(x) || tracked(w) || tracked(z), "linear_act");
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = typed<decltype(linear_act_backward)>("umr::linear_act_backward");
     return op.call(grad, x, w, z, act, slope, nx, nw, nb, nr);
 }
 Tensor balance_loss_backward_once(const Tensor &grad, const Tensor &z, const optional<Tensor> &mask, const Tensor &coef) {
+    no_tangent("the gradient of balance_loss", {&grad, &z, &coef});
     once_only(tracked(grad) || tracked(z) || tracked(coef), "balance_loss");
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = typed<decltype(balance_loss_backward)>("umr::balance_loss_backward");
