@@ -37,3 +37,9 @@ def test_forward_mode_over_a_gradient_is_refused(which):
     leaf, out = (x, UF.linear_act(x, w, activation="tanh")) if which == "linear" else (z, UF.balance_loss(z, _m(5, 1, dtype=torch.int64))[0])
     with fwAD.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         torch.autograd.grad(out, leaf, fwAD.make_dual(torch.ones_like(out).detach(), torch.ones_like(out).detach()))
+
+
+def test_autocast_is_registered_for_the_layer():
+    """(what it does: tests/test_gpu_nn_layers.py)"""
+    UF._nn_ops()
+    assert torch._C._dispatch_has_kernel_for_dispatch_key("umr::linear_act", "AutocastCUDA")

@@ -14,6 +14,7 @@
 //   umr::balance_loss_coef(...) -> (loss, counts, coef)     below autograd
 //   umr::balance_loss_backward(grad, scores, mask, coef) -> Tensor
 #include <ATen/ATen.h>
+#include <ATen/autocast_mode.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -320,6 +321,15 @@ Tensor linear_act_autograd(const Tensor &x, const Tensor &w, const optional<Tens
     return op.call(x, w, b, r, act, slope);
 }
 
+// Under torch.autocast every tensor is cast to its type, as torch's own linear layer does.  (balance_loss takes scores of any type.)
+Tensor linear_act_autocast(const Tensor &x, const Tensor &w, const optional<Tensor> &b, const optional<Tensor> &r, int64_t act, double slope) {
+    c10::impl::ExcludeDispatchKeyGuard below(c10::DispatchKey::AutocastCUDA);
+    static const auto op = typed<decltype(linear_act)>("umr::linear_act");
+    const auto type = at::autocast::get_autocast_dtype(at::kCUDA);
+    const auto cast = [&](const auto &t) { return at::autocast::cached_cast(type, t, at::kCUDA); };
+    return op.call(cast(x), cast(w), cast(b), cast(r), act, slope);
+}
+
 // ---------------------------------------------------------------------------------------------- balance_loss
 void balance_sizes(const Tensor &z, const Tensor &inds, const optional<Tensor> &mask) {
     type_of(z, "balance_loss");
@@ -463,6 +473,7 @@ TORCH_LIBRARY_IMPL(umr, Meta, m) {
     m.impl("balance_loss_coef", balance_loss_coef_meta);
     m.impl("balance_loss_backward", balance_loss_backward_meta);
 }
+TORCH_LIBRARY_IMPL(umr, AutocastCUDA, m) { m.impl("linear_act", linear_act_autocast); }
 TORCH_LIBRARY_IMPL(umr, Autograd, m) {
     m.impl("linear_act", linear_act_autograd);
     m.impl("linear_act_backward", linear_act_backward_once);

@@ -769,7 +769,7 @@ def linear_act(x, weight, bias=None, residual=None, activation="none", slope=0.0
     [N], residual [.., N] or one row [N] for all -> [.., N].  activation: none, relu, leaky_relu (slope >= 0), tanh, gelu (the
     exact form), silu.
 
-    float32, bfloat16 or float16, one type for all; sums are fp32 and a result is rounded once.  Any strides: rows that are
+    float32, bfloat16 or float16, one type for all (torch.autocast casts them to its own); sums are fp32 and a result is rounded once.  Any strides: rows that are
     contiguous are read in place, whatever lies between them.  Gradients to x, weight, bias and residual (in 16 bits the gradient of the
     pre-activation is rounded to 16 bits, as the operands of the matrix unit are); at a kink the derivative is the negative
     side's.  Not differentiable twice, no forward-mode derivative: both are refused.  The same inputs give the same bits in every call.
