@@ -19,14 +19,16 @@ namespace {
 // ------------------------------------------------------------------------------------------------ epilogue
 __host__ __device__ __forceinline__ bool kinked(int act) { return act == UMR_ACT_RELU || act == UMR_ACT_LEAKY_RELU; }
 
-// exp and the normal distribution.  EXACT (fp32 results): the library's functions.  Otherwise (results of 16 bits) exp is one
-// v_exp_f32 and Phi is Abramowitz and Stegun's 7.1.26, which shares its exponential with phi: off by at most 1e-7, where a
-// 16-bit result is off by 2^-11 of itself.
+// exp and the normal distribution, both to a few steps of the value itself, also where Phi is tiny (0.5 (1 + erf) has no digit left
+// at -6).  EXACT (fp32 results): the library's functions.  Otherwise (results of 16 bits) exp is one v_exp_f32, and the tail Phi(-a) =
+// exp(-a^2 / 2) t q(t), t = 1 / (1 + 0.346 a), shares it with phi: q is a minimax fit of degree 6 to the Mills ratio over a <= 14, within
+// 2e-8 of Phi and 7e-6 relative, where half a step of the result is 2^-11 or 2^-8 of it.
 template <bool EXACT> __device__ __forceinline__ float exp_of(float x) { return EXACT ? expf(x) : exp2_of(x * 1.44269504088896341f); }
 template <bool EXACT> __device__ __forceinline__ float normal_cdf(float z, float gauss) {       // gauss = exp(-z^2 / 2)
-    if (EXACT) return 0.5f * (1.f + erff(z * 0.70710678118654752f));
-    const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678118654752f * fabsf(z));
-    const float tail = 0.5f * gauss * (t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))));
+    if (EXACT) return 0.5f * erfcf(z * -0.70710678118654752f);
+    const float t = __builtin_amdgcn_rcpf(1.f + 0.346f * fabsf(z));
+    const float q = 0.138244497f + t * (0.134363111f + t * (0.147132262f + t * (-0.0041666107f + t * (0.229732837f + t * (-0.189794395f + t * 0.0444883194f)))));
+    const float tail = gauss * (t * q);
     return z < 0.f ? tail : 1.f - tail;
 }
 
