@@ -47,7 +47,10 @@ template <bool EXACT> __device__ __forceinline__ float act_slope(float z, int ac
     switch (act) {
         case UMR_ACT_RELU: return z > 0.f ? 1.f : 0.f;
         case UMR_ACT_LEAKY_RELU: return z > 0.f ? 1.f : slope;
-        case UMR_ACT_TANH: { const float t = tanhf(z); return 1.f - t * t; }
+        case UMR_ACT_TANH: {        // 1 - tanh^2 without the difference, which has no digits left where tanh rounds to 1
+            const float e = exp_of<EXACT>(-2.f * fabsf(z)), d = 1.f + e;
+            return 4.f * e / (d * d);
+        }
         case UMR_ACT_GELU: { const float e = exp_of<EXACT>(-0.5f * z * z); return normal_cdf<EXACT>(z, e) + z * e * 0.39894228040143268f; }
         case UMR_ACT_SILU: { const float s = 1.f / (1.f + exp_of<EXACT>(-z)); return s * (1.f + z * (1.f - s)); }
         default: return 1.f;
