@@ -45,7 +45,7 @@ template <bool EXACT> __device__ __forceinline__ float act_value(float z, int ac
 
 template <bool EXACT> __device__ __forceinline__ float act_slope(float z, int act, float slope) {      // act'(z)
     switch (act) {
-        case UMR_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+        case UMR_ACT_RELU: return z <= 0.f ? 0.f : 1.f;            // (a NaN hides no gradient)
         case UMR_ACT_LEAKY_RELU: return z > 0.f ? 1.f : slope;
         case UMR_ACT_TANH: {        // 1 - tanh^2 without the difference, which has no digits left where tanh rounds to 1
             const float e = exp_of<EXACT>(-2.f * fabsf(z)), d = 1.f + e;
