@@ -7,7 +7,8 @@
  *   - a matrix operand is described by its element strides (row, head); its last dimension has stride 1.  Strides of 0 are
  *     allowed in operands that are read (a broadcast), outputs are dense
  *   - outputs and workspaces overlap nothing else of the call (parts of a result may be written twice, with the same bits)
- *   - sizes may be 0 (an empty product is 0); M, N, K < 2^27, G < 65536, M * G * max(N, K) < 2^46
+ *   - sizes may be 0 (an empty product is 0); M, N, K < 2^27, G < 65536, M * G * max(N, K) < 2^46; M * N, M * K and N * K of one head
+ *     < 2^35 (a larger one is UMR_ERR_ARG where its tiles are more than a launch holds)
  */
 #ifndef UMR_NN_H
 #define UMR_NN_H

@@ -34,7 +34,7 @@ def lib():
         os.replace(tmp, SO)
     L = ctypes.CDLL(SO)
     L.nn_route.argtypes = [_I, _L, _L, _L, _I, _I, ctypes.POINTER(_I)]
-    L.nn_run_tile.argtypes = [_I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _P, _L, _L, _P, _P, _L, _L, _L, _I, _I, _F]
+    L.nn_run_tile.argtypes = [_I, _I, _I, _P, _L, _L, _P, _L, _L, _P, _P, _L, _L, _P, _P, _L, _L, _L, _I, _I, _F, _L]
     return L
 
 
@@ -45,7 +45,7 @@ def route(L, direction, M, G, N, K, dtype):
     return L.nn_route(KIND[direction], nq, np, nc, G, H.DTYPE[dtype], ctypes.byref(parts)), parts.value
 
 
-def run_tile(L, direction, tile, x, w, gy, bias=None, res=None, act="none", slope=0.0, want_z=False):
+def run_tile(L, direction, tile, x, w, gy, bias=None, res=None, act="none", slope=0.0, want_z=False, most=0):
     """x [M,G,K], w [G,N,K], gy [M,G,N] of which the direction's two are read -> (output, z or None); margins checked"""
     (M, G, K), N = (x if x is not None else gy).shape, (w if w is not None else gy).shape[1 if w is not None else 2]
     K = (x if x is not None else w).shape[2]
@@ -61,6 +61,8 @@ def run_tile(L, direction, tile, x, w, gy, bias=None, res=None, act="none", slop
     out = H.Guarded(shape, t.dtype, "cpu")
     z = H.Guarded(shape, t.dtype if act in ("relu", "leaky_relu") else torch.float32, "cpu") if want_z else None
     rc = L.nn_run_tile(KIND[direction], tile, H.DTYPE[t.dtype], *P, *Q, None if bias is None else bias.data_ptr(),
-                       *((None, 0, 0) if res is None else rows(res)), out.t.data_ptr(), z.t.data_ptr() if z else None, nq, np, nc, G, H.ACT[act], slope)
-    assert rc == 0 and out.untouched_outside() and (z is None or z.untouched_outside())
+                       *((None, 0, 0) if res is None else rows(res)), out.t.data_ptr(), z.t.data_ptr() if z else None, nq, np, nc, G, H.ACT[act], slope, most)
+    if rc:
+        return rc
+    assert out.untouched_outside() and (z is None or z.untouched_outside())
     return out.t, (z.t if z else None)

@@ -58,3 +58,21 @@ def test_rows_far_apart_take_another_path_to_the_same_bits(dtype):
     for tile in (64, 128, 256) if dtype != torch.float32 else (64, 128):
         assert torch.equal(R.run_tile(L, "forward", tile, x, w, None)[0], R.run_tile(L, "forward", 128, near, w, None)[0])
         assert torch.equal(R.run_tile(L, "weight", tile, x, None, gy)[0], R.run_tile(L, "weight", 128, near, None, gy)[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("direction", list(R.KIND))
+def test_more_heads_than_a_launch_holds(direction, dtype):
+    """a launch's threads are counted in 32 bits, so many heads take several launches (here: of 2 and of 3 heads of 2 x 1 tiles, then of all);
+    a head alone that is more than a launch is refused"""
+    L = R.lib()
+    M, G, N, K = {"forward": (70, 7, 20, 9), "input": (70, 7, 9, 20), "weight": (9, 7, 70, 20)}[direction]
+    x, w, bias, r, gy = C.inputs(M, G, N, K, dtype, "cpu", pad=1)
+    args = {"forward": (x, w, None, bias, r), "input": (None, w, gy), "weight": (x, None, gy)}[direction]
+    for act in (("relu", "gelu") if direction == "forward" else ("none",)):
+        kw = dict(act=act, want_z=direction == "forward")
+        want = R.run_tile(L, direction, 64, *args, **kw)
+        for most in (4, 7, 1000):
+            got = R.run_tile(L, direction, 64, *args, most=most, **kw)
+            assert torch.equal(got[0], want[0]) and (want[1] is None or torch.equal(got[1], want[1]))
+        assert R.run_tile(L, direction, 64, *args, most=1, **kw) == -1

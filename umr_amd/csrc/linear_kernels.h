@@ -801,28 +801,50 @@ __global__ __launch_bounds__(256) void k_linear_act_grad(const T *__restrict__ g
 }
 
 template <class T> __global__ __launch_bounds__(256) void k_linear_colsum(const float *part, int blocks, T *db, T *dr, long cols) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= cols) return;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < cols; i += (long)gridDim.x * 256) {
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        T *out = which ? dr : db;
-        if (!out) continue;
-        float s = 0.f;
+        for (int which = 0; which < 2; ++which) {
+            T *out = which ? dr : db;
+            if (!out) continue;
+            float s = 0.f;
 #pragma unroll 8
-        for (int b = 0; b < blocks; ++b) s += part[((long)b * 2 + which) * cols + i];
-        out[i] = from_f32<T>(s);
+            for (int b = 0; b < blocks; ++b) s += part[((long)b * 2 + which) * cols + i];
+            out[i] = from_f32<T>(s);
+        }
     }
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-template <class T, int NQ, int NP, int FQ, int FP> int launch_tile(int kind, const Product &pr, const Epilogue &e, hipStream_t st) {
-    const long tq = ceil_div(pr.nq, NQ * FQ * 32), tp = ceil_div(pr.np, NP * FP * 32), grid = tq * tp * pr.S * pr.G;
-    if (tq * tp > 0x7fffffffL || grid > 0x7fffffffL) return UMR_ERR_ARG;
+// the product from head g0 on (not of a split contraction: its parts lie head by head in one plane)
+template <class T> void from_head(Product &pr, Epilogue &e, long g0) {
+    pr.P.data = (const T *)pr.P.data + g0 * pr.P.head;
+    pr.Q.data = (const T *)pr.Q.data + g0 * pr.Q.head;
+    if (e.bias) e.bias = (const T *)e.bias + g0 * pr.np;
+    if (e.res) e.res = (const T *)e.res + g0 * e.r_head;
+    e.out = (T *)e.out + g0 * e.o_head;
+    if (e.z && kinked(e.act)) e.z = (T *)e.z + g0 * e.o_head;
+    else if (e.z) e.z = (float *)e.z + g0 * e.o_head;
+}
+
+// `most`: workgroups of a launch, whose threads are counted in 32 bits.  More heads than fit take several launches.
+template <class T, int NQ, int NP, int FQ, int FP>
+int launch_tile(int kind, const Product &all, const Epilogue &epilogue, hipStream_t st, long most = 0xffffffffL / (64 * NQ * NP)) {
+    const long tq = ceil_div(all.nq, NQ * FQ * 32), tp = ceil_div(all.np, NP * FP * 32), head = tq * tp * all.S;
+    const long at_once = most / head < all.G ? most / head : all.G;
+    if (at_once < 1 || (at_once < all.G && all.S > 1)) return UMR_ERR_ARG;
     constexpr int NT = 64 * NQ * NP;
-    if (kind == FORWARD) UMR_LAUNCH((k_linear_tile<T, false, false, NQ, NP, FQ, FP>), (unsigned)grid, NT, 0, st, pr, e, (int)tq, (int)tp);
-    else if (kind == GRAD_INPUT) UMR_LAUNCH((k_linear_tile<T, true, false, NQ, NP, FQ, FP>), (unsigned)grid, NT, 0, st, pr, e, (int)tq, (int)tp);
-    else UMR_LAUNCH((k_linear_tile<T, true, true, NQ, NP, FQ, FP>), (unsigned)grid, NT, 0, st, pr, e, (int)tq, (int)tp);
-    return umr_launch_status();
+    for (long g0 = 0; g0 < all.G; g0 += at_once) {
+        Product pr = all;
+        Epilogue e = epilogue;
+        from_head<T>(pr, e, g0);
+        pr.G = (int)(all.G - g0 < at_once ? all.G - g0 : at_once);
+        const unsigned grid = (unsigned)(head * pr.G);
+        if (kind == FORWARD) UMR_LAUNCH((k_linear_tile<T, false, false, NQ, NP, FQ, FP>), grid, NT, 0, st, pr, e, (int)tq, (int)tp);
+        else if (kind == GRAD_INPUT) UMR_LAUNCH((k_linear_tile<T, true, false, NQ, NP, FQ, FP>), grid, NT, 0, st, pr, e, (int)tq, (int)tp);
+        else UMR_LAUNCH((k_linear_tile<T, true, true, NQ, NP, FQ, FP>), grid, NT, 0, st, pr, e, (int)tq, (int)tp);
+        if (umr_launch_status() != UMR_OK) return UMR_ERR_LAUNCH;
+    }
+    return UMR_OK;
 }
 
 template <class T, int QT> int launch_few(int kind, const Product &pr, const Epilogue &e, hipStream_t st) {
@@ -868,8 +890,8 @@ template <class T> int run_act_grad(const ActGrad &a, hipStream_t st) {
                a.G, a.rows, a.act, a.slope);
     if (umr_launch_status() != UMR_OK) return UMR_ERR_LAUNCH;
     if (a.part) {
-        const long cols = a.G * a.N;
-        UMR_LAUNCH((k_linear_colsum<T>), (unsigned)ceil_div(cols, 256), 256, 0, st, (const float *)a.part, (int)a.blocks, (T *)a.db, (T *)a.dr, cols);
+        const long cols = a.G * a.N, work = ceil_div(cols, 256);
+        UMR_LAUNCH((k_linear_colsum<T>), (unsigned)(work < 8192 ? work : 8192), 256, 0, st, (const float *)a.part, (int)a.blocks, (T *)a.db, (T *)a.dr, cols);
     }
     return umr_launch_status();
 }
