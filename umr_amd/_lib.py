@@ -107,6 +107,8 @@ def lib():
         h.umr_version.restype = ctypes.c_char_p
         h.umr_build_id.restype = ctypes.c_char_p
         for name, (argtypes, restype) in list(SIGNATURES.items()) + list(SIGNATURES_NN.items()):
+            if name in SIGNATURES_NN and not hasattr(h, name):
+                continue                                  # an experimental build of the render path alone (tools/build_variant.py)
             fn = getattr(h, name)
             fn.argtypes = argtypes
             fn.restype = restype
