@@ -32,3 +32,18 @@ def test_layers_under_autocast(dtype):
     for cast in (False, True):
         with torch.autocast("cuda", dtype=dtype, enabled=cast), pytest.raises(RuntimeError, match="float32, bfloat16|weight is"):
             UF.linear_act(x.double(), net[0].weight.double())
+
+
+def test_fused_net_with_an_activation_that_is_changed_in_place():
+    from umr_amd import model as M
+    torch.manual_seed(1)
+    net = nn.Sequential(nn.Linear(5, 6), nn.LeakyReLU(0.2), nn.ReLU(inplace=True)).to(DEV)
+    x = torch.randn(7, 5, device=DEV)
+    want = net(x)
+    M.fuse_linears(net)
+    y = net(x)
+    # sums of 5 products and a bias, and two roundings: at most 9 u of their magnitudes on either side
+    mag = x.abs() @ net[0].weight.detach().abs().t() + net[0].bias.detach().abs()
+    assert bool(((y - want).detach().abs() <= 2 * 9 * 2.0 ** -24 * mag).all())
+    y.square().sum().backward()
+    assert bool(torch.isfinite(net[0].weight.grad).all()) and float(net[0].weight.grad.abs().sum()) > 0

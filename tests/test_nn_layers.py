@@ -227,3 +227,13 @@ def test_folded_cameras_keep_the_networks_type_and_scales(dtype):
             assert a.dtype == b.dtype == dtype
             if dtype is torch.float64:                                       # (sums in another order)
                 assert float((a - b).abs().max()) <= 1e-13 * max(1.0, float(a.abs().max()))
+
+
+@pytest.mark.parametrize("after", [nn.Dropout(0.5, inplace=True), nn.ReLU(inplace=True)], ids=str)
+def test_fused_net_keeps_a_leaky_relu_whose_output_the_next_module_changes_in_place(after):
+    """on the GPU the fused layer keeps its output for the backward call, so changing it raises; nn.LeakyReLU keeps its input"""
+    net = nn.Sequential(nn.Linear(5, 6), nn.LeakyReLU(0.2), copy.deepcopy(after))
+    fused = M.fuse_linears(copy.deepcopy(net))
+    assert fused[0].activation == "none" and type(fused[1]) is nn.LeakyReLU
+    net[2].inplace = False
+    assert M.fuse_linears(net)[0].activation == "leaky_relu"

@@ -107,16 +107,17 @@ def fuse_linears(net):
     Left as it is, with what follows it: a layer of any other class (a subclass of nn.Linear, a layer with a parametrization).  A
     layer that is registered in several places applies no activation itself: another place may have another one behind it.  A
     Sequential with a forward of its own keeps its LeakyReLUs: what follows what is not known there.  So does a pair whose values
-    between product and activation a hook asks for; one registered later sees the activated output."""
+    between product and activation a hook asks for (one registered later sees the activated output), and one whose output the next
+    module changes in place: the fused layer keeps it for its backward call."""
     uses = Counter(kid for m in net.modules() for kid in m._modules.values())
     for m in list(net.modules()):
         if type(m) is nn.Linear:
             m.__class__ = Linear
     for m in list(net.modules()):
         kids = _chains(m)
-        for (_, a), (name, b) in zip(kids, kids[1:]):
+        for (_, a), (name, b), (_, c) in zip(kids, kids[1:], kids[2:] + [("", None)]):
             if type(a) is Linear and a.activation == "none" and uses[a] == 1 and type(b) is nn.LeakyReLU and b.negative_slope >= 0 and \
-                    not _hooked(a, inputs_too=False) and not _hooked(b):
+                    not _hooked(a, inputs_too=False) and not _hooked(b) and not getattr(c, "inplace", False):
                 a.activation, a.slope = "leaky_relu", float(b.negative_slope)
                 m._modules[name] = nn.Identity()
     return net
