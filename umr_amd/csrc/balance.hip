@@ -10,8 +10,9 @@
 // that a wave reads whole lines whatever E is; the softmax's maximum and sum are butterflies over those lanes, in fp32.  Forward: a
 // lane adds up its columns over its rows in registers, lanes and waves meet in a fixed order, choices are counted with integer
 // LDS atomics; one workgroup joins the workgroups' parts in part order (in double).  Nothing depends on the order of arrival.
-// 2^19 x 128 bf16 with 8 choices a row: rows 53 us (168 MB, 3.2 TB/s: the exponentials are next), fold and join 5 each, backward 65 us
-// (268 MB, 4.1 TB/s).
+// 2^19 x 128 bf16 with 8 choices a row: rows 53 us (168 MB, 3.2 TB/s), fold and join 5 each, backward 64 us (268 MB, 4.2 TB/s).  In the
+// rows the vector unit is busy 63 % of the time (the exponentials alone are 7 us of it) and the waves wait 61 % of theirs: a row's loads
+// start when the one before is done.
 #include "nn_common.h"
 
 namespace {
@@ -280,8 +281,8 @@ __global__ __launch_bounds__(WG) void k_balance_backward(const T *__restrict__ z
     }
 
 long rows_per_group(long T, int E) {
-    // a workgroup's 16 waves take 16 KB of 16-bit or fp32 scores at a time, at least twice; at most 512 workgroups, whose parts one
-    // workgroup joins
+    // a workgroup's 16 waves take 16 bytes a lane, 16 KB of scores, at a time: at least twice in fp32, once in 16 bits; at most 512
+    // workgroups, whose parts one workgroup joins
     long rows = (T + 511) / 512, least = 32768 / (4 * (E < 4 ? 4 : E));
     if (least < 32) least = 32;
     return rows < least ? least : rows;

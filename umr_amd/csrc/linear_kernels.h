@@ -126,9 +126,10 @@ template <class T> __global__ __launch_bounds__(256) void k_linear_join(Epilogue
 // the same bits); a matrix smaller than a tile repeats its last row, whose results are dropped.  A last step that is not whole
 // loads 16 bytes that end with the row and moves them into place, and zeros behind them, when they go to LDS.
 //
-// 256 x 256 (16 bits): 8 waves of 128 x 64, one workgroup a CU; bf16 8192 x 4096 x 4096 forward 310 us (890 TFLOP/s), with gelu, z and
-// residual 394; dx 355 - 407, dw 340.  The matrix unit is busy 38 % of the time: LDS carries 256 KB a step and the loads' latency shows.
-// 128 x 128: fp32 4096^3 1170 us (117 TFLOP/s, matrix unit 74 % busy).  64 x 64 where larger tiles would leave CUs idle.
+// 256 x 256 (16 bits): 8 waves of 128 x 64, one workgroup a CU; bf16 8192 x 4096 x 4096 forward with gelu, z and residual 394 us (698
+// TFLOP/s), dx 406, dw 350.  The matrix unit is busy 30, 28 and 32 % of the time and the waves wait 47, 53 and 38 % of theirs: LDS carries
+// 256 KB a step and the loads' latency shows.  128 x 128: fp32 4096^3 1180 us (116 TFLOP/s, matrix unit 74 % busy).  64 x 64 where larger
+// tiles would leave CUs idle: fp32 10000 x 1011 x 350 93 us (49 % busy).
 constexpr int ROW_BYTES = 144;
 constexpr long NEAR = 1L << 22;                               // rows closer than this many elements: a tile's offsets fit 32 bits
 
@@ -733,7 +734,7 @@ template <int N> struct Count { static constexpr int value = N; };
 
 // One pass over gy and z.  A wave takes 256 columns (4 a lane) of the rows r0 + wave, r0 + wave + 4, ...; sums meet in LDS, and
 // over the row blocks in k_linear_colsum, both in a fixed order.  The lanes at the right edge take the last 4 columns, some of them
-// twice, so that every load is 4 wide and none is behind a branch.  8192 x 4096 gelu in bf16: 60 us, 268 MB at 4.5 TB/s.
+// twice, so that every load is 4 wide and none is behind a branch.  8192 x 4096 gelu in bf16: 61 us, 268 MB at 4.4 TB/s.
 template <class T>
 __global__ __launch_bounds__(256) void k_linear_act_grad(const T *__restrict__ gy, long g_row, long g_head, const void *__restrict__ z, T *__restrict__ dz, T *db, T *dr, float *part,
                                                          long M, long N, int G, long rows, int act, float slope) {
@@ -763,7 +764,10 @@ __global__ __launch_bounds__(256) void k_linear_act_grad(const T *__restrict__ g
             if (dz) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) gv[k][i] *= act_slope<sizeof(T) == 4>(zv[k][i], act, slope);
-                // dz in the operator's own type: the operand of both gradient products (16-bit matrix instructions take 16 bits)
+                // dz in the operator's own type: the operand of both gradient products (16-bit matrix instructions take 16 bits).
+                // This second rounding puts dx and dw 1.4 times as far from 64 bits as their own rounding alone would (bf16 2.35e-3
+                // against 1.66e-3 in the norm, fp16 2.9e-4 against 2.1e-4; a layer that rounds z too, 2.42e-3 and 3.0e-4); the halves of
+                // an fp32 dz would take both products twice.  The sums over the rows have it in fp32.
                 store4(dz + ((m + 4 * k) * G + g) * N + n, wide, gv[k]);
             }
 #pragma unroll

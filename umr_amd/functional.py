@@ -772,7 +772,7 @@ def linear_act(x, weight, bias=None, residual=None, activation="none", slope=0.0
     float32, bfloat16 or float16, one type for all (torch.autocast casts them to its own); sums are fp32 and a result is rounded once.  Any strides: rows that are
     contiguous are read in place, whatever lies between them.  Gradients to x, weight, bias and residual (in 16 bits the gradient of the
     pre-activation is rounded to 16 bits, as the operands of the matrix unit are); at a kink the derivative is the negative
-    side's.  Not differentiable twice, no forward-mode derivative: both are refused.  The same inputs give the same bits in every call.
+    side's (its side is the pre-activation's in the type: in 16 bits one that rounds to 0 is at the kink).  Not differentiable twice, no forward-mode derivative: both are refused.  The same inputs give the same bits in every call.
     Fewer than 2^27 rows, columns and inputs; tensors on the current device, work on its current stream."""
     op, _, table = _nn_ops(x, weight, bias, residual)
     if weight.dim() != 2:
@@ -798,7 +798,7 @@ def balance_loss(scores, inds, mask=None):
 
     loss is a float32 scalar, 1 when all choices are used alike, differentiable once in scores (through P; counts are constants; no forward mode);
     counts [E] int64.  A score of -inf is never chosen; a row of nothing else counts as masked out; masked rows may hold
-    anything.  An index outside 0 .. E-1 counts for no choice, one that appears twice counts twice.  E <= 1024."""
+    anything.  An index outside 0 .. E-1 counts for no choice, one that appears twice counts twice.  E <= 1024, T k < 2^31."""
     _, op, _ = _nn_ops(scores, inds, mask)
     return op(scores, inds, mask)
 
