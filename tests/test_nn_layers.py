@@ -237,3 +237,33 @@ def test_fused_net_keeps_a_leaky_relu_whose_output_the_next_module_changes_in_pl
     assert fused[0].activation == "none" and type(fused[1]) is nn.LeakyReLU
     net[2].inplace = False
     assert M.fuse_linears(net)[0].activation == "leaky_relu"
+
+
+def test_a_forward_of_an_instances_own_is_respected():
+    """module.forward replaced on the instance, as offloading wrappers do it: on a layer, its LeakyReLU, the Sequential, a camera"""
+    torch.manual_seed(10)
+    x = torch.randn(7, 5).double()
+
+    def replaced(m):
+        old = m.forward
+        m.forward = lambda v: old(v) + 1
+        return m
+    for where in (0, 1, 2, None):
+        def build():
+            torch.manual_seed(11)
+            net = nn.Sequential(nn.Linear(5, 5).double(), nn.LeakyReLU(0.2), _normed(5)).eval()
+            if where is None:
+                return replaced(net)
+            replaced(net[where])
+            return net
+        assert torch.equal(build()(x), M.fuse_linears(build())(x)), where
+
+        def folding():
+            torch.manual_seed(12)
+            net = nn.Sequential(nn.Linear(5, 5).double(), _normed(5), nn.LeakyReLU(0.2)).eval()
+            replaced(net if where is None else net[where])
+            return net
+        assert torch.allclose(folding()(x), M.fold_for_inference(folding())(x), rtol=0, atol=1e-12), where
+    net = _predictor()
+    replaced(net.camera_predictor[1])
+    _same_cameras(net, M.fold_for_inference(net), torch.randn(6, 12).double())

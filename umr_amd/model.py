@@ -92,12 +92,13 @@ class Linear(nn.Linear):
 
 def _chains(m):
     """[(name, child)] of a Sequential that calls its children one after the other, [] of any other module."""
-    return list(m._modules.items()) if isinstance(m, nn.Sequential) and type(m).forward is nn.Sequential.forward else []
+    own = "forward" in vars(m) or type(m).forward is not nn.Sequential.forward
+    return list(m._modules.items()) if isinstance(m, nn.Sequential) and not own else []
 
 
 def _hooked(m, inputs_too=True):
-    """A hook looks at this module's output or gradient (inputs_too: or at its input)."""
-    return bool(m._forward_hooks or m._backward_hooks or m._backward_pre_hooks or inputs_too and m._forward_pre_hooks)
+    """A hook looks at this module's output or gradient (inputs_too: or at its input), or the instance has a forward of its own."""
+    return bool(m._forward_hooks or m._backward_hooks or m._backward_pre_hooks or inputs_too and m._forward_pre_hooks or "forward" in vars(m))
 
 
 def fuse_linears(net):
